@@ -13,7 +13,9 @@ What is different here:
   tables, so a group of windowed layers can give back the pages its window has
   passed while a group of full-attention layers keeps all of them.
 * A page id addresses all cache layers of its group at once; the pool of a
-  group is ``[pages, cache layers, planes (k,v), kv heads, page size, head dim]``.
+  group is ``[pages, cache layers, planes (k,v), kv heads, page size, head dim]``,
+  or, held in 4 bits (``packed``), bytes ``[pages, cache layers, planes, kv heads,
+  slab]`` (a slab is a page's rows of one head: csrc/packed.cuh).
 * Every live request also holds a **slot**: an index into fixed-size
   per-request state: on the device its length, last token, sampling
   parameters and block tables (:class:`pagedserve_b200.cache.slots.SlotStore`,
@@ -75,6 +77,14 @@ class KVNeed:
         if self.chunk is not None:
             return length - length % self.chunk
         return 0
+
+    def page_numbers(self, page_size: int, packed: bool = False) -> int:
+        """What a page of one cache layer takes: numbers of the compute type, or bytes where it is ``packed``."""
+        if packed:
+            from pagedserve_b200.kernels.ops import packed_slab_bytes
+
+            return self.planes * self.n_kv_heads * packed_slab_bytes(page_size, self.head_dim)
+        return self.planes * self.n_kv_heads * page_size * self.head_dim
 
     def merged(self, other: "KVNeed") -> Optional["KVNeed"]:
         """The need of a cache layer that two runs with different masks read (one of them writes it): the same
@@ -163,8 +173,9 @@ class CacheGroup:
     """Layers with the same :class:`KVNeed`: one pool, one free list, one set of tables."""
 
     def __init__(self, need: KVNeed, cache_layers: Sequence[int], page_size: int, num_pages: int,
-                 max_pages_per_request: int, dtype=None, device=None, scratch_pages: int = 0):
+                 max_pages_per_request: int, dtype=None, device=None, scratch_pages: int = 0, packed: bool = False):
         self.need = need
+        self.packed = packed                        # held in 4 bits
         self.cache_layers = list(cache_layers)      # global cache-layer ids, in pool order
         self.page_size = page_size
         self.num_pages = num_pages
@@ -180,15 +191,18 @@ class CacheGroup:
                 raise CacheError("a cache layer has one or two planes")
             shape = (num_pages + scratch_pages, len(self.cache_layers), need.planes, need.n_kv_heads, page_size,
                      need.head_dim)
+            if packed:
+                slab = need.page_numbers(page_size, packed=True) // (need.planes * need.n_kv_heads)
+                shape, dtype = (*shape[:4], slab), torch.uint8
             self.pool = torch.empty(shape, dtype=dtype, device=device)
 
-    # strides in elements, used by the kernels
+    # strides in elements (bytes where the group is packed), used by the kernels
     @property
     def page_stride(self) -> int:
-        return len(self.cache_layers) * self.need.planes * self.need.n_kv_heads * self.page_size * self.need.head_dim
+        return len(self.cache_layers) * self.need.page_numbers(self.page_size, self.packed)
 
     def layer_views(self, cache_layer: int):
-        """(k, v) views ``[pages, kv heads, page size, head dim]`` of one cache layer (the same view twice
+        """(k, v) views ``[pages, kv heads, page size, head dim]`` (packed: ``[pages, kv heads, slab]``) of one cache layer (the same view twice
         where the layer has a single plane)."""
         local = self.cache_layers.index(cache_layer)
         return self.pool[:, local, 0], self.pool[:, local, self.need.planes - 1]
@@ -212,7 +226,7 @@ class CacheManager:
 
     def __init__(self, kv_needs: Sequence[Optional[KVNeed]], state_needs: Sequence[Optional[StateNeed]],
                  page_size: int, num_pages: int, max_slots: int, max_model_len: int,
-                 dtype=None, device=None, scratch_tokens: int = 0):
+                 dtype=None, device=None, scratch_tokens: int = 0, packed: bool = False):
         if page_size <= 0 or (page_size & (page_size - 1)) or page_size > 64:
             raise CacheError("page_size must be a power of two, at most 64")
         if max_slots <= 0:
@@ -223,6 +237,7 @@ class CacheManager:
         self.max_pages_per_request = -(-max_model_len // page_size)
         self.device = device
         self.dtype = dtype
+        self.packed = packed                                 # keys and values held in 4 bits
 
         by_need: Dict[KVNeed, List[int]] = {}
         for layer, need in enumerate(kv_needs):
@@ -234,7 +249,8 @@ class CacheManager:
         scratch_pages = -(-self.scratch_tokens // page_size)
         self.scratch_slot = max_slots
         self.groups: List[CacheGroup] = [
-            CacheGroup(need, layers, page_size, num_pages, self.max_pages_per_request, dtype, device, scratch_pages)
+            CacheGroup(need, layers, page_size, num_pages, self.max_pages_per_request, dtype, device, scratch_pages,
+                       packed)
             for need, layers in by_need.items()
         ]
         # the device copy of every slot's state: lengths, sampling parameters, block tables by slot

@@ -1,7 +1,7 @@
 """Engine-level settings: everything that is not part of the model itself.
 
 Counterpart of the arguments of the reference's ``build_scheduler``
-(reference: main.py:136-150) with the backend switch and INT8 cache removed.
+(reference: main.py:136-150) with the backend switch removed and a cache of 4 bits in place of the INT8 one.
 """
 
 from __future__ import annotations
@@ -12,6 +12,7 @@ from typing import Optional
 from pagedserve_b200.config.registry import ConfigError
 
 SUPPORTED_DTYPES = ("float32", "bfloat16")
+SUPPORTED_KV_CACHE_DTYPES = ("model", "int4")   # the execution dtype, or 4 bits a number (csrc/packed.cuh)
 # A model without a position table has no longest request of its own; block tables need some width.
 UNBOUNDED_MODEL_LEN = 32768
 ORCA_STRATEGY = "orca"
@@ -34,11 +35,14 @@ class EngineConfig:
     enable_cuda_graphs: bool = True             # reference: --disable-cuda-graphs, main.py:317-321
     max_model_len: Optional[int] = None         # longest request; None: the model's own bound, or
                                                 # UNBOUNDED_MODEL_LEN for a model that has none
+    kv_cache_dtype: str = "model"               # reference: --kv-cache-dtype, main.py:311-316
     device: str = "cuda:0"
 
     def __post_init__(self):
         if self.dtype not in SUPPORTED_DTYPES:
             raise ConfigError(f"unknown dtype {self.dtype!r}; choose one of {SUPPORTED_DTYPES}")
+        if self.kv_cache_dtype not in SUPPORTED_KV_CACHE_DTYPES:
+            raise ConfigError(f"unknown KV cache dtype {self.kv_cache_dtype!r}; choose one of {SUPPORTED_KV_CACHE_DTYPES}")
         if self.block_size <= 0 or self.block_size > 64 or (self.block_size & (self.block_size - 1)):
             raise ConfigError("block_size must be a power of two between 1 and 64")
         if self.num_blocks is not None and self.num_blocks <= 0:

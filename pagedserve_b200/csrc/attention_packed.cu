@@ -1,0 +1,236 @@
+// Attention of single tokens over a cache held in 4 bits, on CUDA cores (packed.cuh has the cache's format): float32, and every
+// head size up to 256.
+//
+// A key reads as low_j + step_j c in group j, so that
+//   q . k = sum over j of step_j (q_j . c_j) + low_j sum(q_j)           (q_j, c_j: the numbers and codes of group j)
+// and the weighted values are sum over keys of (p step_j) c + sum over keys of p low_j: a code is met by one multiply-add, the group's two numbers once a key.
+// A code is put into the mantissa of 16.0 (a rotation and a mask: 16 + c exactly) and moved to the middle of its range, c - 8, with low_j + 8 step_j
+// in place of low_j: sums of 16 + c, eight times as large, cost the float32 results a digit (5 tokens, 512 keys, heads of 64: 2.4e-6 off, so
+// 3e-7).  Scores, weights, sums: float32.
+//
+// A CTA has a token, a head and a share of its keys: tiles of 32 keys aligned to absolute positions, one tile after another for each
+// warp.  For the scores a lane has a key, for the values the numbers `lane` of every group.  The shares of a token and head are a
+// thread-block cluster and merge through shared memory, in the order of the shares.
+#include "packed.cuh"
+
+namespace ps {
+namespace packed {
+
+constexpr int WARPS = 4, TILE = 32;
+
+// number i of a word as code - 8: `rotation` brings the code to bits 19 .. 22
+__device__ __forceinline__ float centred(uint32_t word, int rotation) {
+    return __uint_as_float((__funnelshift_l(word, word, rotation) & 0x00780000u) | 0x41800000u) - 24.f;
+}
+__host__ __device__ __forceinline__ int rotation_of(int i) { return (19 - code_shift(i)) & 31; }
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(WARPS * 32)
+tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ out, long long out_stride, int wide,
+              const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
+              const int* __restrict__ token_row, const int* __restrict__ positions, Pages pages, int n_heads, int n_kv_heads, int head_dim,
+              int window, float scale, float softcap, const float* __restrict__ sink) {
+    constexpr int NUMBERS = NG * GROUP;
+    __shared__ __align__(16) float q_s[NUMBERS];           // in the order of the cache's words
+    __shared__ float sum_s[NG];                             // of each group's queries
+    __shared__ float weight_s[WARPS][TILE][NG];
+    __shared__ long long row_s[WARPS][TILE];
+    __shared__ float acc_s[WARPS][NUMBERS], m_s[WARPS], l_s[WARPS];
+    __shared__ float share_acc[NUMBERS], share_ml[2];
+    pdl_prologue();
+    q = pdl_fresh(q);
+    k_pool = pdl_fresh(k_pool);
+    v_pool = pdl_fresh(v_pool);
+    const int t = blockIdx.x, h = blockIdx.y, share = blockIdx.z, shares = gridDim.z, g = h / (n_heads / n_kv_heads);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int p = positions[t], lo = p < 0 ? 0 : first_visible_key(p, window), table_row = token_row[t];
+    const int last = min(p, (pages.bt_stride << pages.page_log2) - 1);          // (what is beyond the table has no page)
+    for (int i = threadIdx.x; i < NUMBERS; i += WARPS * 32) {
+        const int place = i >> 3, d = place % NG * GROUP + place / NG * 8 + (i & 7);
+        q_s[i] = d < head_dim ? to_float(q[t * q_stride + h * head_dim + d]) : 0.f;
+    }
+    __syncthreads();
+    if (threadIdx.x < NG) {
+        float sum = 0.f;
+        for (int i = 0; i < NUMBERS; ++i)
+            if ((i >> 3) % NG == (int)threadIdx.x) sum += q_s[i];
+        sum_s[threadIdx.x] = sum;
+    }
+    __syncthreads();
+    float q_sum[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) q_sum[j] = sum_s[j];
+
+    const int page_size = 1 << pages.page_log2, words_at = page_size * NG * 16;
+    const long long head_at = (long long)g * slab_bytes(page_size, head_dim);
+    const float scale_log2 = scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.f, acc[NG], lows[NG];       // acc: number `lane` of every group; l and lows: this lane's keys
+#pragma unroll
+    for (int j = 0; j < NG; ++j) acc[j] = lows[j] = 0.f;
+    const int my_rotation = (19 - code_shift(lane & 7)) & 31, my_part = lane >> 3;
+    for (int tile = lo / TILE + share * WARPS + warp; tile * TILE <= last; tile += shares * WARPS) {
+        const int key = tile * TILE + lane;
+        const bool seen = key >= lo && key <= last;
+        const int page = seen ? pages.of(table_row, key) : -1;
+        const long long at = page < 0 ? -1 : (long long)page * page_stride + head_at;
+        const int row = key & (page_size - 1);
+        float s = -INFINITY;
+        if (page >= 0) {
+            const uint4* codes = reinterpret_cast<const uint4*>(k_pool + at) + row * NG;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pool + at + words_at) + row * NG;
+            float dot[NG];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) dot[j] = 0.f;
+#pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                const uint4 raw = codes[u];
+                const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    constexpr int LAST = NG;
+                    const int place = u * 4 + w;
+                    const float4 a = *reinterpret_cast<const float4*>(q_s + place * 8), b = *reinterpret_cast<const float4*>(q_s + place * 8 + 4);
+                    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    float sum = dot[place % LAST];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum = fmaf(centred(word[w], rotation_of(i)), x[i], sum);
+                    dot[place % LAST] = sum;
+                }
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const uint32_t two = words[j];
+                sum = fmaf(step_of(two), dot[j], fmaf(fmaf(8.f, step_of(two), low_of(two)), q_sum[j], sum));
+            }
+            s = softcap > 0.f ? softcap * 1.4426950408889634f * tanhf(sum * (scale / softcap)) : sum * scale_log2;
+        }
+        const float m_new = fmaxf(m, warp_max(s)), base = m_new == -INFINITY ? 0.f : m_new, shrink = exp2f(m - base);
+        m = m_new;
+        const float weight = page >= 0 ? exp2f(s - base) : 0.f;
+        l = fmaf(l, shrink, weight);
+        row_s[warp][lane] = page < 0 ? -1 : at + row * NG * 16;
+        if (page >= 0) {
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + at + words_at) + row * NG;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const uint32_t two = words[j];
+                const float step = step_of(two);
+                weight_s[warp][lane][j] = weight * step;
+                lows[j] = fmaf(lows[j], shrink, weight * fmaf(8.f, step, low_of(two)));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NG; ++j) lows[j] *= shrink;
+        }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) acc[j] *= shrink;
+        __syncwarp();
+#pragma unroll 4
+        for (int k = 0; k < TILE; ++k) {
+            const long long from = row_s[warp][k];
+            if (from < 0) continue;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + from) + my_part * NG;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) acc[j] = fmaf(centred(words[j], my_rotation), weight_s[warp][k][j], acc[j]);
+        }
+        __syncwarp();
+    }
+    // the warps' states, then the shares'
+    l = warp_sum(l);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) acc_s[warp][j * GROUP + lane] = acc[j] + warp_sum(lows[j]);
+    if (lane == 0) { m_s[warp] = m; l_s[warp] = l; }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, m_s[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total = fmaf(l_s[w], exp2f(m_s[w] - base), total);
+    for (int d = threadIdx.x; d < NUMBERS; d += WARPS * 32) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) sum = fmaf(acc_s[w][d], exp2f(m_s[w] - base), sum);
+        share_acc[d] = sum;
+    }
+    if (threadIdx.x == 0) { share_ml[0] = top; share_ml[1] = total; }
+    if (shares > 1) cluster_sync_all();
+    else __syncthreads();
+    if (share == 0) {
+        const float sink_log2 = sink ? sink[h] * 1.4426950408889634f : -INFINITY;
+        float all = sink_log2;
+        for (int c = 0; c < shares; ++c) all = fmaxf(all, shares > 1 ? ld_cluster_f32(&share_ml[0], c) : share_ml[0]);
+        const float ground = all == -INFINITY ? 0.f : all;
+        float denominator = sink ? exp2f(sink_log2 - ground) : 0.f;
+        for (int c = 0; c < shares; ++c) {
+            const float m_c = shares > 1 ? ld_cluster_f32(&share_ml[0], c) : share_ml[0], l_c = shares > 1 ? ld_cluster_f32(&share_ml[1], c) : share_ml[1];
+            denominator = fmaf(l_c, exp2f(m_c - ground), denominator);
+        }
+        for (int d = threadIdx.x; d < head_dim; d += WARPS * 32) {
+            float sum = 0.f;
+            for (int c = 0; c < shares; ++c) {
+                const float m_c = shares > 1 ? ld_cluster_f32(&share_ml[0], c) : share_ml[0], a_c = shares > 1 ? ld_cluster_f32(&share_acc[d], c) : share_acc[d];
+                sum = fmaf(a_c, exp2f(m_c - ground), sum);
+            }
+            // (no key at all: zero; a NaN stays one)
+            const float result = denominator == 0.f ? sum * 0.f : sum / denominator;
+            const long long to = t * out_stride + h * head_dim + d;
+            if (wide) reinterpret_cast<float*>(out)[to] = result;
+            else reinterpret_cast<T*>(out)[to] = from_float<T>(result);
+        }
+    }
+    if (shares > 1) cluster_sync_all();                     // the shares stay until they were read
+}
+
+template <typename T, int NG>
+int launch_tokens(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
+                  long long page_stride, const int* token_row, const int* positions, const Pages& pages, int tokens, int n_heads, int n_kv_heads,
+                  int head_dim, int window, float scale, float softcap, const float* sink, int shares, cudaStream_t s) {
+    return launch_pdl_cluster(tokens_kernel<T, NG>, dim3(tokens, n_heads, shares), dim3(WARPS * 32), 0, s, shares, (const T*)q, q_stride, out,
+                              out_stride, wide, (const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, token_row, positions, pages,
+                              n_heads, n_kv_heads, head_dim, window, scale, softcap, sink);
+}
+
+}  // namespace packed
+}  // namespace ps
+
+// q / out: rows of n_heads * head_dim numbers; token t stands at positions[t] (below 0: its row of `out` becomes zero) and reads the pages of
+// row token_row[t] of block_table (bt_stride wide; what has no page is not seen).  window, softcap, sink as in ps_paged_attention_simt.
+// out_dtype: that of q, or float32.  shares: 1, 2, 4 or 8 CTAs for the keys of a token and head.
+PS_EXPORT int ps_packed_tokens_simt(const void* q, long long q_stride, void* out, long long out_stride, int out_dtype, const void* k_pool,
+                                    const void* v_pool, int n_pages, long long page_stride, const int* token_row, const int* positions,
+                                    const int* block_table, int bt_stride, int tokens, int n_heads, int n_kv_heads, int head_dim, int page_size,
+                                    int window, float scale, float softcap, const float* sink, int shares, int dtype, void* stream) {
+    using namespace ps::packed;
+    if (tokens <= 0) return PS_OK;
+    if (!q || !out || !k_pool || !v_pool || !token_row || !positions || !block_table) return PS_ERR_BAD_ARGUMENT;
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return PS_ERR_BAD_ARGUMENT;
+    if (!sizes_ok(n_kv_heads, head_dim, page_size) || n_heads > 65535) return PS_ERR_UNSUPPORTED;
+    if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
+    if (shares != 1 && shares != 2 && shares != 4 && shares != 8) return PS_ERR_BAD_ARGUMENT;
+    if ((dtype != PS_F32 && dtype != PS_BF16) || (out_dtype != dtype && out_dtype != PS_F32)) return PS_ERR_UNSUPPORTED;
+    const Pages pages = {block_table, bt_stride, n_pages, log2_of(page_size)};
+    const int wide = dtype == PS_BF16 && out_dtype == PS_F32;
+#define PS_PACKED_TOKENS(NG)                                                                                                                       \
+    case NG:                                                                                                                                       \
+        return dtype == PS_F32 ? launch_tokens<float, NG>(q, q_stride, out, out_stride, wide, k_pool, v_pool, page_stride, token_row, positions,   \
+                                                          pages, tokens, n_heads, n_kv_heads, head_dim, window, scale, softcap, sink, shares,      \
+                                                          (cudaStream_t)stream)                                                                    \
+                               : launch_tokens<__nv_bfloat16, NG>(q, q_stride, out, out_stride, wide, k_pool, v_pool, page_stride, token_row,      \
+                                                                  positions, pages, tokens, n_heads, n_kv_heads, head_dim, window, scale, softcap, \
+                                                                  sink, shares, (cudaStream_t)stream)
+    switch (groups_of(head_dim)) {
+        PS_PACKED_TOKENS(1);
+        PS_PACKED_TOKENS(2);
+        PS_PACKED_TOKENS(3);
+        PS_PACKED_TOKENS(4);
+        PS_PACKED_TOKENS(5);
+        PS_PACKED_TOKENS(6);
+        PS_PACKED_TOKENS(7);
+        PS_PACKED_TOKENS(8);
+    }
+#undef PS_PACKED_TOKENS
+    return PS_ERR_UNSUPPORTED;
+}

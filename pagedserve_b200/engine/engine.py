@@ -14,7 +14,7 @@ import torch
 from pagedserve_b200.cache.budget import MIB, kv_cache_budget, pages_for_budget
 from pagedserve_b200.cache.manager import CacheManager
 from pagedserve_b200.config.engine_config import UNBOUNDED_MODEL_LEN, EngineConfig
-from pagedserve_b200.config.registry import ModelConfig, load_config_dict, resolve_architecture
+from pagedserve_b200.config.registry import ConfigError, ModelConfig, load_config_dict, resolve_architecture
 from pagedserve_b200.engine.step import ModelRunner
 from pagedserve_b200.kernels.ops import Ops
 from pagedserve_b200.models.model import Model
@@ -82,12 +82,18 @@ class Engine:
         state_needs = self.model.state_needs()
         width = torch.empty(0, dtype=self.dtype).element_size()
         # bytes one page costs summed over the groups (each group has its own pool of equal page count)
+        packed = cfg.kv_cache_dtype == "int4"
+        if packed:
+            unable = sorted({type(block.mixer).__name__ for block in self.model.blocks
+                             if block.mixer.cache_need() is not None and not block.mixer.packs_cache})
+            if unable:
+                raise ConfigError(f"kv_cache_dtype 'int4' is not built for {', '.join(unable)}: these layers keep a cache of their own kind")
+            width = 1
         by_need: Dict[object, int] = {}
         for need in kv_needs:
             if need is not None:
                 by_need[need] = by_need.get(need, 0) + 1
-        bytes_per_page = sum(need.planes * count * need.n_kv_heads * need.head_dim * cfg.block_size * width
-                             for need, count in by_need.items())
+        bytes_per_page = sum(count * need.page_numbers(cfg.block_size, packed) * width for need, count in by_need.items())
         self.bytes_per_block = bytes_per_page
         if cfg.num_blocks is not None:
             num_pages = cfg.num_blocks
@@ -104,7 +110,7 @@ class Engine:
                                          cfg.block_size)
         return CacheManager(kv_needs, state_needs, cfg.block_size, int(num_pages), cfg.max_num_seqs,
                             self.spec.max_model_len, dtype=self.dtype, device=self.device,
-                            scratch_tokens=ModelRunner.PAD_LONG)
+                            scratch_tokens=ModelRunner.PAD_LONG, packed=packed)
 
     # ------------------------------------------------------------------ the calls a user makes
     @property
@@ -139,6 +145,24 @@ class Engine:
 
     def sample(self, logits, temperatures, seeds, positions) -> List[int]:
         return self.sampler.sample(logits, temperatures, seeds, positions)
+
+    def logprobs(self, logits: torch.Tensor, tokens: Sequence[int], top: int = 0):
+        """Log probabilities of ``tokens`` under rows of logits that a step returned, with the entropy of each row's
+        distribution and its ``top`` most likely tokens (:class:`pagedserve_b200.kernels.ops.TokenLogprobs`, on the device).
+        A token of -1 is none."""
+        tokens = [int(token) for token in tokens]
+        if len(tokens) != logits.shape[0]:
+            raise ValueError("one token per row of logits")
+        if any(not -1 <= token < self.vocab_size for token in tokens):
+            raise ValueError(f"a token is outside the vocabulary of {self.vocab_size}")
+        return self.ops.token_logprobs(logits, torch.tensor(tokens, dtype=torch.int32).to(logits.device), top)
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0):
+        """What the model says about given texts: for each prompt a :class:`pagedserve_b200.engine.score.PromptScore` with the log
+        probability of every token behind the first, the entropy and the ``top`` most likely tokens at its place."""
+        from pagedserve_b200.engine.score import score
+
+        return score(self, prompts, top)
 
     def make_scheduler(self, **kwargs):
         from pagedserve_b200.engine.scheduler import Scheduler

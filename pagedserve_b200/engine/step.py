@@ -436,6 +436,27 @@ class ModelRunner:
             raise StepError(f"model returned {logits.shape[0]} logits rows, expected {expected}")
         return logits
 
+    def score(self, entries: Sequence[StepEntry], targets: Sequence[int], top: int = 0):
+        """Run one step; returns what the head says about ``targets``, one token per wanted place in the order of the entries
+        and of their ``want`` lists (:class:`pagedserve_b200.kernels.ops.TokenLogprobs`).  The step's logits never exist as a whole."""
+        entries = [e if isinstance(e, StepEntry) else StepEntry(*e) for e in entries]
+        if len(targets) != sum(len(entry.want) for entry in entries):
+            raise StepError("one target per wanted place")
+        if len(targets) and not (-1 <= min(targets) and max(targets) < self.vocab_size):
+            raise StepError(f"a target is outside the vocabulary of {self.vocab_size}")
+        ctx = self.prepare(entries)
+        try:
+            if len(targets):
+                ctx.scoring = (torch.tensor(targets, dtype=torch.int32).to(self.device), top)
+            result = self._forward(ctx)
+        except Exception:
+            self._abandon(entries)
+            raise
+        self.cache.commit_many([entry.request for entry in entries])
+        self.steps += 1
+        self.tokens_run += ctx.num_tokens
+        return result if len(targets) else None
+
     # ------------------------------------------------------------------ decode-only steps
     def decode(self, entries: Sequence[StepEntry], temperatures, seeds, steps: int = 1) -> np.ndarray:
         """``decode_tokens`` for entries of one token each."""

@@ -10,6 +10,7 @@ an error.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -21,6 +22,8 @@ _DTYPE_CODE = {torch.float32: PS_F32, torch.bfloat16: PS_BF16}
 WEIGHTS_READY = 4             # in linear_simt's ``accumulate``: the weights were complete before the kernel in front began
 COLUMN_FACTOR = 2             # in a product's ``accumulate``: its vector multiplies the columns instead of being added
 _ACT_CODE = {None: 0, "none": 0, "gelu_tanh": 1, "gelu_erf": 2, "relu_squared": 3, "silu": 4, "tanh": 5}
+PACKED_GROUP, PACKED_MAX_HEAD = 32, 256       # of a cache held in 4 bits: numbers that share a scale; the largest head
+MOST_ALTERNATIVES = 32        # most likely tokens that ``token_logprobs`` gives
 _STATUS = {1: "bad argument", 2: "unsupported size or dtype", 3: "kernel launch failed"}
 
 _c_void_p = ctypes.c_void_p
@@ -130,6 +133,12 @@ _SIGNATURES = {
         "ps_host_free": [_P],
         "ps_copy_h2d": [_P, _P, _L, _P],
     },
+    "packed": {
+        "ps_kv_append_packed": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P],
+        "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P],
+        "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
+        "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
+    },
     "bf16": {
         "ps_gemm_skinny_block": [_I, _I, _I],
         "ps_gemm_skinny": [_P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I,
@@ -196,10 +205,25 @@ def _check(status: int, what: str):
         raise KernelError(f"{what}: {_STATUS.get(status, f'status {status}')}")
 
 
+def packed_slab_bytes(page_size: int, head_dim: int) -> int:
+    """Bytes that a page of one key/value head takes in a cache held in 4 bits (csrc/packed.cuh)."""
+    groups = -(-head_dim // PACKED_GROUP)
+    return -(-page_size * groups * 20 // 16) * 16
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype not in _DTYPE_CODE:
         raise KernelError(f"unsupported dtype {dtype}")
     return _DTYPE_CODE[dtype]
+
+
+class TokenLogprobs(NamedTuple):
+    """What :meth:`Ops.token_logprobs` and :meth:`Ops.head_logprobs` return, of each row of logits."""
+
+    logprob: torch.Tensor          # float32 [rows], of the given token
+    entropy: torch.Tensor          # float32 [rows], of the distribution, in nats
+    top_logprobs: torch.Tensor     # float32 [rows, top], the largest log probabilities, largest first
+    top_ids: torch.Tensor          # int32 [rows, top], their tokens
 
 
 class StepArena:
@@ -280,10 +304,12 @@ class Ops:
         self.core = _declare(_load_library("core"), "core")
         self.fast = _declare(_load_library("bf16"), "bf16") if dtype == torch.bfloat16 else None
         self._tc = None              # tcgen05 library, loaded when a product first needs it
+        self._packed = None          # library of the packed cache and of log probabilities, likewise
         self.status = None
         self._counters = None        # zeroed int32 scratch of the split attention kernel
         self.launches = 0            # count of kernel launches issued through this object
         self.arena = None            # a StepArena once a runner has attached one: see ``empty``
+        self._ramps = {}             # device -> int32 0, 1, 2, ... (see ``_counting``)
 
     def empty(self, shape, dtype, device):
         """An uninitialised tensor that lives until the next step begins (from the step arena if a runner
@@ -675,7 +701,7 @@ class Ops:
     def linear_qkv(self, a, w, bias, out, ctx, layer, q_width, kv_width, head_dim, scatter=True):
         """The packed q|k|v projection.  Returns True when the key and value columns were written into
         the pages by the product's own epilogue (then no separate cache write is needed)."""
-        if scatter and layer.k_pool is not None and self.dtype == torch.bfloat16 and head_dim % 16 == 0:
+        if scatter and layer.k_pool is not None and self.dtype == torch.bfloat16 and head_dim % 16 == 0 and not self.packed(layer):
             if hasattr(a, "materialize") and self._fused_norm_ok(a, w):
                 self.linear_skinny_fused(a, w, bias, out, kv=(ctx, layer, q_width, kv_width, head_dim))
                 return True
@@ -1090,6 +1116,8 @@ class Ops:
             if window:
                 raise KernelError("attention: a window or a chunked mask, not both")
             window = -int(chunk)
+        if self.packed(layer):
+            return self._packed_attention(q, k, v, out, ctx, layer, n_heads, n_kv_heads, head_dim, window, scale, write_cache, softcap, sink, mix)
         if write_cache:
             self.kv_append(k, v, ctx.token_slot, ctx.positions, layer.block_table, layer.k_pool, layer.v_pool,
                            layer.page_stride, n_kv_heads, head_dim, layer.page_size)
@@ -1110,6 +1138,251 @@ class Ops:
             return out if mix is None else self.head_mix(every, mix, out, n_heads, n_kv_heads, head_dim)
         return tensorcore.attention(self, q, out, ctx, layer, n_heads, n_kv_heads, head_dim, window, scale,
                                     softcap=softcap, sink=sink, mix=mix)
+
+    # ------------------------------------------------------------------ a cache held in 4 bits
+    def _packed_library(self):
+        if self._packed is None:
+            self._packed = _declare(_load_library("packed"), "packed")
+        return self._packed
+
+    @staticmethod
+    def packed(layer):
+        """Whether a layer's pages hold 4 bits a number."""
+        return layer is not None and layer.k_pool is not None and layer.k_pool.dtype is torch.uint8
+
+    def _append_step(self, k, v, ctx, layer, n_kv_heads, head_dim):
+        self.kv_append_packed(k, v, ctx.token_slot, ctx.positions, layer.block_table, layer.k_pool, layer.v_pool, layer.page_stride,
+                              n_kv_heads, head_dim, layer.page_size)
+
+    def _turn_and_pack(self, turn_keys, k, v, ctx, layer, n_kv_heads, head_dim):
+        """Keys turned in place and both planes written; ``v`` None: the values are the keys before they are turned."""
+        if v is None:
+            self._append_step(None, k, ctx, layer, n_kv_heads, head_dim)
+        turn_keys()
+        self._append_step(k, v, ctx, layer, n_kv_heads, head_dim)
+
+    def _packed_attention(self, q, k, v, out, ctx, layer, n_heads, n_kv_heads, head_dim, window, scale, write_cache, softcap, sink, mix):
+        """The step's attention over a packed cache: short entries token by token, prompt portions in blocks (``tensorcore.attention``
+        cuts a step alike); head sizes that no prompt kernel takes go token by token, too."""
+        if mix is not None:
+            raise KernelError("attention: mixed heads do not read a cache held in 4 bits")
+        if write_cache:
+            self._append_step(k, v, ctx, layer, n_kv_heads, head_dim)
+        pools = (layer.k_pool, layer.v_pool, layer.page_stride)
+        sizes = (n_heads, n_kv_heads, head_dim, layer.page_size, window, scale)
+        short, long_items = ctx.num_short_tokens, ctx.num_items - ctx.num_short_items
+        if long_items and not self.packed_prompts_ok(q, out, head_dim, ctx.num_long_blocks):
+            short, long_items = ctx.num_tokens, 0
+        if short:
+            self.packed_attention_tokens(q[:short], out[:short], *pools, ctx.token_slot, ctx.positions, layer.block_table, *sizes, ctx.max_kv_len,
+                                         softcap=softcap, sink=sink)
+        if long_items:
+            self.packed_attention_prompts(q, out, *pools, ctx.q_start, ctx.kv_len, layer.block_table, ctx.item_slot, ctx.num_short_items,
+                                          long_items, ctx.num_long_blocks, ctx.max_kv_len, *sizes, softcap=softcap, sink=sink)
+        return out
+
+    # The checks of these entry points cost the host as much as a launch if each names what is wrong as it goes: one condition says
+    # whether all is well, and only where it is not does the function behind it find out what.
+    def _packed_pools(self, what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table):
+        """Checks what the kernels over a packed cache (csrc/packed.cuh) share; the pages of the pools."""
+        if not (0 < head_dim <= PACKED_MAX_HEAD) or page_size not in (1, 2, 4, 8, 16, 32, 64):
+            raise KernelError(f"{what}: head sizes up to {PACKED_MAX_HEAD}, pages of a power of two up to 64 tokens")
+        slab = packed_slab_bytes(page_size, head_dim)
+        shape, strides, device = k_pool.shape, (page_stride, slab, 1), k_pool.get_device()
+        if not (len(shape) == 3 and shape[1] == n_kv_heads and shape[2] == slab and k_pool.stride() == strides and v_pool.shape == shape
+                and v_pool.stride() == strides and k_pool.dtype is torch.uint8 and v_pool.dtype is torch.uint8 and page_stride % 16 == 0
+                and block_table.dtype is torch.int32 and block_table.ndim == 2 and block_table.is_contiguous()
+                and device >= 0 and device == v_pool.get_device() == block_table.get_device() and device == _device_number()):
+            self._explain_pools(what, k_pool, v_pool, page_stride, n_kv_heads, slab, block_table)
+        return shape[0]
+
+    def _explain_pools(self, what, k_pool, v_pool, page_stride, n_kv_heads, slab, block_table):
+        for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
+            _require(pool, name, torch.uint8)
+            if pool.ndim != 3 or pool.shape[1:] != (n_kv_heads, slab) or pool.shape[0] != k_pool.shape[0]:
+                raise KernelError(f"{what}: {name} must be [pages, {n_kv_heads}, {slab}] bytes")
+            if pool.stride()[1:] != (slab, 1) or (pool.shape[0] > 1 and pool.stride(0) != page_stride):
+                raise KernelError(f"{what}: the slabs of {name} must lie behind one another, its pages page_stride bytes apart")
+            if page_stride % 16:
+                raise KernelError(f"{what}: pages are a multiple of 16 bytes apart")
+        _require(block_table, "block_table", torch.int32)
+        if block_table.ndim != 2 or not block_table.is_contiguous():
+            raise KernelError(f"{what}: block_table must be contiguous rows of page ids")
+        for tensor in (k_pool, v_pool, block_table):
+            self._on_current_device(what, tensor)
+
+    def _indices(self, what, count, device, **tensors):
+        for name, tensor in tensors.items():
+            if not (tensor.dtype is torch.int32 and tensor.ndim == 1 and tensor.numel() >= count and tensor.is_contiguous()
+                    and tensor.get_device() == device):
+                _require(tensor, name, torch.int32)
+                self._on_current_device(what, tensor)
+                raise KernelError(f"{what}: {name} must be {count} contiguous int32")
+
+    @staticmethod
+    def _on_current_device(what, tensor):
+        if tensor.get_device() != _device_number():
+            raise KernelError(f"{what}: a tensor is on {tensor.device}, which is not the current device")
+
+    def _packed_rows(self, what, name, rows, count, width, device, dtypes):
+        if not (rows.ndim == 2 and rows.shape == (count, width) and rows.stride(1) == 1 and rows.dtype in dtypes and rows.get_device() == device):
+            _require(rows, name)
+            self._on_current_device(what, rows)
+            raise KernelError(f"{what}: {name} must be {count} rows of {width} numbers in {' or '.join(map(str, dtypes))}")
+
+    def kv_append_packed(self, k_src, v_src, token_row, positions, block_table, k_pool, v_pool, page_stride, n_kv_heads, head_dim,
+                         page_size):
+        """Round this step's K/V rows ([T, n_kv_heads * head_dim] views of the compute type) to 4 bits and write them into their pages:
+        what :meth:`kv_append` is for a cache of the compute type.  ``k_pool`` / ``v_pool`` uint8 [pages, n_kv_heads, slab]
+        (:func:`packed_slab_bytes`), ``page_stride`` in bytes.  Token t goes to row ``token_row[t]`` of ``block_table``; one with a
+        position below 0 or without a page is left out.  ``k_src`` or ``v_src`` None leaves that plane as it is."""
+        what = "kv_append_packed"
+        given = [(name, src) for name, src in (("k", k_src), ("v", v_src)) if src is not None]
+        if not given:
+            raise KernelError(f"{what}: no rows")
+        n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
+        T = given[0][1].shape[0]
+        device = k_pool.get_device()
+        for name, src in given:
+            self._packed_rows(what, name, src, T, n_kv_heads * head_dim, device, (self.dtype,))
+        self._indices(what, T, device, token_row=token_row, positions=positions)
+        self.launches += 1
+        _check(self._packed_library().ps_kv_append_packed(
+            _ptr(k_src), k_src.stride(0) if k_src is not None else 0, _ptr(v_src), v_src.stride(0) if v_src is not None else 0,
+            _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], _ptr(k_pool), _ptr(v_pool), n_pages, page_stride, T,
+            n_kv_heads, head_dim, page_size, self.code, _stream()), what)
+
+    def kv_unpack(self, k_pool, v_pool, page_stride, kv_len, block_table, item_row, first_item, n_items, span, out, n_kv_heads, head_dim,
+                  page_size):
+        """What a packed cache holds of items ``first_item ..``, as pages of the compute type: ``out`` [n_items * span / P, 2, n_kv_heads, P,
+        head_dim], contiguous, P a power of two that divides ``span``.  Position p of the i-th of these items goes to page i * span / P +
+        p / P; positions from ``kv_len`` of the item (or ``span``) on are left as they are.  ``item_row``: the block-table row of each item."""
+        what = "kv_unpack"
+        n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
+        _require(out, "out", self.dtype)
+        if n_items <= 0 or span <= 0 or first_item < 0:
+            raise KernelError(f"{what}: no items")
+        if (out.ndim != 5 or not out.is_contiguous() or out.shape[1:3] != (2, n_kv_heads) or out.shape[4] != head_dim
+                or out.shape[3] <= 0 or out.shape[3] & (out.shape[3] - 1) or span % out.shape[3]
+                or out.shape[0] < n_items * (span // out.shape[3])):
+            raise KernelError(f"{what}: out must be [items * span / P, 2, n_kv_heads, P, head_dim]")
+        self._on_current_device(what, out)
+        self._indices(what, first_item + n_items, k_pool.get_device(), kv_len=kv_len, item_row=item_row)
+        self.launches += 1
+        _check(self._packed_library().ps_kv_unpack(
+            _ptr(k_pool), _ptr(v_pool), n_pages, page_stride, _ptr(kv_len) + 4 * first_item, _ptr(block_table), block_table.shape[1],
+            _ptr(item_row) + 4 * first_item, n_items, span, _ptr(out), out.shape[3], n_kv_heads, head_dim, page_size, self.code, _stream()), what)
+        return out
+
+    def _packed_queries(self, what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device):
+        if n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads:
+            raise KernelError(f"{what}: n_heads must be a multiple of n_kv_heads")
+        rows = q.shape[0]
+        self._packed_rows(what, "q", q, rows, n_heads * head_dim, device, (self.dtype,))
+        self._packed_rows(what, "out", out, rows, n_heads * head_dim, device, (self.dtype, torch.float32))
+        if softcap is not None and not softcap > 0:
+            raise KernelError(f"{what}: softcap must be positive")
+        if sink is not None and not (sink.dtype is torch.float32 and sink.numel() == n_heads and sink.is_contiguous() and sink.get_device() == device):
+            _require(sink, "sink", torch.float32)
+            self._on_current_device(what, sink)
+            raise KernelError(f"{what}: one sink per query head")
+        return rows
+
+    def packed_attention_tokens(self, q, out, k_pool, v_pool, page_stride, token_row, positions, block_table, n_heads, n_kv_heads, head_dim,
+                                page_size, window, scale, max_kv_len, softcap=None, sink=None):
+        """Attention of single tokens over a packed cache: token t, at ``positions[t]``, reads the pages of row ``token_row[t]`` of
+        ``block_table``.  ``max_kv_len`` bounds every token's context (it fixes the grid, so a CUDA graph passes the longest).  ``out`` may be float32
+        in bfloat16.  A token at a position below 0 sees nothing: its row becomes zero.  Otherwise as :meth:`paged_attention_decode`."""
+        what = "packed_attention_tokens"
+        n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
+        device = k_pool.get_device()
+        T = self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device)
+        self._indices(what, T, device, token_row=token_row, positions=positions)
+        if T == 0:
+            return out
+        shares = 1
+        tiles = -(-int(max_kv_len) // 128)
+        while shares < 8 and T * n_heads * shares * 2 <= 2 * 148 * 8 and shares * 2 <= tiles:
+            shares *= 2
+        self.launches += 1
+        _check(self._packed_library().ps_packed_tokens_simt(
+            _ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(out.dtype), _ptr(k_pool), _ptr(v_pool), n_pages, page_stride,
+            _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim, page_size,
+            window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, self.code, _stream()), what)
+        return out
+
+    UNPACKED_BYTES = 512 << 20        # most scratch that prompts take whose rows are unpacked first (but one item's rows always)
+
+    def _counting(self, count, device):
+        """int32 0, 1, 2, ...: at least ``count`` of them.  (Never written again, and kept: captured graphs may read it.)"""
+        kept = self._ramps.setdefault(device, [])
+        if not kept or kept[-1].numel() < count:
+            kept.append(torch.arange(max(4096, 2 * count), dtype=torch.int32, device=device))
+        return kept[-1]
+
+    def packed_attention_prompts(self, q, out, k_pool, v_pool, page_stride, q_start, kv_len, block_table, item_row, first_item, n_items,
+                                 max_blocks, max_kv_len, n_heads, n_kv_heads, head_dim, page_size, window, scale, softcap=None, sink=None):
+        """Causal attention of prompt portions over a packed cache: items ``first_item ..`` of the step, ``max_blocks`` >= the number of 64-query
+        blocks they make up, ``max_kv_len`` >= their contexts.  ``q`` / ``out`` are the step's flat token arrays; item i's tokens are rows
+        ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  Otherwise as
+        :meth:`prefill_attention`."""
+        what = "packed_attention_prompts"
+        self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
+        device = k_pool.get_device()
+        self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device)
+        if first_item < 0 or n_items < 0:
+            raise KernelError(f"{what}: items below 0")
+        self._indices(what, first_item + n_items, device, kv_len=kv_len, item_row=item_row)
+        self._indices(what, first_item + n_items + 1, device, q_start=q_start)
+        device = k_pool.device
+        if n_items == 0 or max_blocks <= 0 or max_kv_len <= 0:
+            return out
+        if not self.packed_prompts_ok(q, out, head_dim, max_blocks):
+            raise KernelError(f"{what}: heads of {head_dim} in {self.dtype} with these strides go token by token (packed_attention_tokens)")
+        # The rows as pages of the compute type, some items at a time, and the kernel for those.
+        page = 64
+        span = min(-(-int(max_kv_len) // page) * page, -(-block_table.shape[1] * page_size // page) * page)
+        item_bytes = span * 2 * n_kv_heads * head_dim * self.dtype.itemsize
+        at_once = max(1, min(n_items, self.UNPACKED_BYTES // item_bytes))
+        scratch = self.empty((at_once * (span // page), 2, n_kv_heads, page, head_dim), self.dtype, device)
+        counting = self._counting(at_once * (span // page), device)
+        table = counting[:at_once * (span // page)].view(at_once, span // page)
+        for start in range(first_item, first_item + n_items, at_once):
+            count = min(at_once, first_item + n_items - start)
+            self.kv_unpack(k_pool, v_pool, page_stride, kv_len, block_table, item_row, start, count, span, scratch, n_kv_heads, head_dim, page_size)
+            self._prompts_from_pages(q, out, scratch, q_start[start:], kv_len[start:], table, counting, count, max_blocks, n_heads, n_kv_heads,
+                                     head_dim, page, window, scale, softcap, sink)
+        return out
+
+    def packed_prompts_ok(self, q, out, head_dim, max_blocks):
+        """Whether :meth:`packed_attention_prompts` takes these rows: float32 heads of up to 128 numbers in whole 16-byte pieces, bfloat16 ones
+        in multiples of 16 up to 128."""
+        if self.dtype == torch.float32:
+            return (head_dim % 4 == 0 and head_dim <= 128 and max_blocks <= 65535 and q.stride(0) % 4 == 0 and out.stride(0) % 4 == 0
+                    and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+        return head_dim % 16 == 0 and head_dim <= 128 and max_blocks <= 65535 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+
+    def _prompts_from_pages(self, q, out, pool, q_start, kv_len, table, item_row, n_items, max_blocks, n_heads, n_kv_heads, head_dim, page,
+                            window, scale, softcap, sink):
+        """Prompt portions over pages of the compute type ([pages, 2, kv heads, page, head size])."""
+        k_pool, v_pool, stride = pool[:, 0], pool[:, 1], pool.stride(0)
+        rest = (n_heads, n_kv_heads, head_dim, page, window or 0, scale)
+        if self.dtype == torch.float32:
+            arguments = (_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pool), _ptr(v_pool), stride, _ptr(q_start), _ptr(kv_len),
+                         _ptr(table), table.stride(0), _ptr(item_row), 0, n_items)
+            last = (*rest, float(softcap or 0.0), _ptr(sink), 0)
+            self.launches += 1
+            if self.F32_TC_HEADS[0] <= head_dim <= self.F32_TC_HEADS[1]:
+                _check(self._tc_library().ps_prompt_attention_f32_tc(*arguments, (max_blocks + n_items) // 2, *last,
+                                                                     _ptr(self.status_flag(q.device)), _stream()), "prompt_attention_f32_tc")
+            else:
+                _check(self.core.ps_prompt_attention_f32(*arguments, max_blocks, *last, _stream()), "prompt_attention_f32")
+            return
+        pieces = dict(item_row=item_row, softcap=softcap, sink=sink)
+        if self.prefill_tc_ok(head_dim, page, q, out, pool):
+            self.prefill_attention_tc(q, out, pool.unsqueeze(1), 0, q_start, kv_len, table, 0, n_items, (max_blocks + n_items) // 2, *rest, **pieces)
+        else:
+            self.prefill_attention(q, out, k_pool, v_pool, stride, q_start, kv_len, table, 0, n_items, max_blocks, *rest, **pieces)
 
     # ------------------------------------------------------------------ rotary positions + cache write
     def rotary_cache_write(self, q, k, v, inv_freq, rot_dims, interleaved, ctx, layer, n_heads, n_kv_heads,
@@ -1133,6 +1406,12 @@ class Ops:
         if q.shape[1] != n_heads * head_dim or k.shape[1] != n_kv_heads * head_dim:
             raise KernelError("rotary: widths do not match the head counts")
         pools = write_cache and layer is not None and layer.k_pool is not None
+        if pools and self.packed(layer):
+            # the keys are turned where they lie, as the queries are, and rounded on their way into the pages
+            turn = lambda rows, heads: self.rotary_cache_write(rows, rows, None, inv_freq, rot_dims, interleaved, ctx, None, heads, heads, head_dim,
+                                                               write_cache=False)
+            turn(q, n_heads)
+            return self._turn_and_pack(lambda: turn(k, n_kv_heads), k, v, ctx, layer, n_kv_heads, head_dim)
         if pools:
             _require(layer.k_pool, "k_pool", self.dtype)
         self.launches += 1
@@ -1175,6 +1454,13 @@ class Ops:
         if q.stride(1) != 1 or q.shape[1] != n_heads * head_dim:
             raise KernelError("head_norm_rotary: queries must be rows of n_heads * head_dim")
         pools = write_cache and k is not None and layer is not None and layer.k_pool is not None
+        if pools and self.packed(layer):
+            turn = lambda rows, gain, heads: self.head_norm_rotary_cache_write(
+                rows, None, None, gain, None, eps, inv_freq, rot_dims, interleaved, dim, ctx, None, heads, heads, head_dim, write_cache=False,
+                amplitude=amplitude)
+            turn(q, q_gain, n_heads)
+            same = v.data_ptr() == k.data_ptr()               # values that are the keys as projected
+            return self._turn_and_pack(lambda: turn(k, k_gain, n_kv_heads), k, None if same else v, ctx, layer, n_kv_heads, head_dim)
         if pools:
             _require(layer.k_pool, "k_pool", self.dtype)
         self.launches += 1
@@ -1980,6 +2266,64 @@ class Ops:
         return inner
 
     # ------------------------------------------------------------------ sampling
+    def _logprob_results(self, what, rows, vocabulary, targets, top, device):
+        _require(targets, "targets", torch.int32)
+        if targets.ndim != 1 or targets.numel() != rows or not targets.is_contiguous() or targets.device != device:
+            raise KernelError(f"{what}: one int32 token per row, on the device of the rows")
+        if not (0 <= top <= min(vocabulary, MOST_ALTERNATIVES)):
+            raise KernelError(f"{what}: top is 0 to {MOST_ALTERNATIVES}, and at most the vocabulary")
+        self._on_current_device(what, targets)
+        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)
+        return TokenLogprobs(new((rows,), torch.float32), new((rows,), torch.float32), new((rows, top), torch.float32), new((rows, top), torch.int32))
+
+    def token_logprobs(self, logits, targets, top=0, status=None, results=None):
+        """:class:`TokenLogprobs` of float32 ``logits`` [rows, vocabulary] and one token a row (int32): its log probability under the row's softmax,
+        the distribution's entropy, and the ``top`` largest log probabilities with their tokens (of equal logits the lower token first).
+        A token of -1 is none: its log probability is 0.  A token outside the vocabulary sets the status flag and gives NaN.
+        -infinity is a token of probability 0; a NaN or +infinity in a row makes the row's numbers NaN.  ``results``: tensors to write to."""
+        what = "token_logprobs"
+        _require(logits, "logits", torch.float32)
+        if logits.ndim != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
+            raise KernelError(f"{what}: logits must be rows of a vocabulary")
+        rows, V = logits.shape
+        results = results or self._logprob_results(what, rows, V, targets, top, logits.device)
+        if rows == 0:
+            return results
+        ld = logits.stride(0) if rows > 1 else V
+        if ld < V:
+            raise KernelError(f"{what}: the rows of logits overlap")
+        if status is None:
+            status = self.status_flag(logits.device)
+        self.launches += 1
+        _check(self._packed_library().ps_token_logprobs(_ptr(logits), ld, rows, V, _ptr(targets), top, _ptr(results.logprob), _ptr(results.entropy),
+                                           _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), what)
+        return results
+
+    LOGITS_AT_ONCE = 1 << 24          # logits that stay in L2 between the product and what is read from them
+
+    def head_logprobs(self, x, table, targets, top=0, status=None):
+        """:meth:`token_logprobs` of the logits ``x @ table.T`` (operands of the compute type, logits in float32), some rows at a time: all
+        logits at once never exist."""
+        what = "head_logprobs"
+        if hasattr(x, "materialize"):
+            x = x.materialize()
+        _require(x, "x", self.dtype)
+        _require(table, "table", self.dtype)
+        if x.ndim != 2 or table.ndim != 2 or x.shape[1] != table.shape[1] or table.shape[0] == 0 or x.shape[1] == 0:
+            raise KernelError(f"{what}: shapes do not match: x {tuple(x.shape)} table {tuple(table.shape)}")
+        if x.stride(1) != 1 or table.stride(1) != 1 or x.device != table.device:
+            raise KernelError(f"{what}: x and table must be rows on one device")
+        rows, V = x.shape[0], table.shape[0]
+        results = self._logprob_results(what, rows, V, targets, top, x.device)
+        at_once = max(128, self.LOGITS_AT_ONCE // V // 128 * 128)
+        logits = self.empty((min(rows, at_once), V), torch.float32, x.device)
+        for start in range(0, rows, at_once):
+            end = min(rows, start + at_once)
+            part = logits[:end - start]
+            self.linear(x[start:end], table, None, part)
+            self.token_logprobs(part, targets[start:end], top, status, TokenLogprobs(*(result[start:end] for result in results)))
+        return results
+
     def sample(self, logits, temperature, seed, position, out, pos_offset=0):
         """out[r] = argmax (temperature 0) or a Gumbel-max draw keyed by (seed[r], position[r] + pos_offset);
         logits float32 [R, V]."""

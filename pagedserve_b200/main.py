@@ -10,8 +10,10 @@ folder with ``config.json`` and ``model.safetensors``, or the name of a size
 seeded random weights.  ``--decode-attention-backend`` names the implementation of
 single-token attention as in the reference (main.py:305-310); this engine has one, its
 own paged kernels (``cuda``), and says so when it is asked for ``torch`` or ``triton``.
-``--kv-cache-dtype`` is ``model`` (main.py:311-316); ``int8`` is refused: quantised
-caches are not built.  Prompts are token ids: there is no tokenizer in the engine.
+``--kv-cache-dtype`` is ``model`` or ``int4`` (main.py:311-316); the reference's ``int8`` is refused: the quantised
+cache of this engine holds 4 bits a number.  Prompts are token ids: there is no tokenizer in the engine.
+``--score`` generates nothing: it prints the log probability of every prompt token behind the first, the entropy at its
+place and, with ``--top-logprobs N``, the N most likely tokens there.
 """
 
 from __future__ import annotations
@@ -32,7 +34,7 @@ from pagedserve_b200.config.engine_config import (
 # reference: main.py:27-28. "cuda" is this engine's only implementation; the reference's two names are accepted
 # and answered with a note, so that its command lines keep working.
 SUPPORTED_DECODE_ATTENTION_BACKENDS = ("cuda", "torch", "triton")
-SUPPORTED_KV_CACHE_DTYPES = ("model", "int8")
+SUPPORTED_KV_CACHE_DTYPES = ("model", "int4", "int8")
 
 
 def build_engine(model: str, seed: int = 0, **engine_options):
@@ -73,8 +75,8 @@ def build_scheduler(model: str = "tiny-a", scheduling_strategy: str = ORCA_STRAT
     if kv_cache_dtype not in SUPPORTED_KV_CACHE_DTYPES:                          # reference: main.py:165-167
         raise ValueError(f"Unknown KV cache dtype '{kv_cache_dtype}'. "
                          f"Choose one of: {', '.join(SUPPORTED_KV_CACHE_DTYPES)}")
-    if kv_cache_dtype != "model":
-        raise ValueError("KV cache dtype 'int8' is not built: the cache is kept in the execution dtype")
+    if kv_cache_dtype == "int8":
+        raise ValueError("KV cache dtype 'int8' is not built: the cache is kept in the execution dtype ('model') or in 4 bits ('int4')")
     if max_batch_size is None:
         max_batch_size = 32                                  # reference: main.py:181-182 (CUDA default)
     if max_batch_size <= 0:
@@ -84,7 +86,8 @@ def build_scheduler(model: str = "tiny-a", scheduling_strategy: str = ORCA_STRAT
                           kv_cache_memory_utilization=kv_cache_memory_utilization,
                           kv_cache_safety_mb=kv_cache_safety_mb, max_num_seqs=max_batch_size,
                           max_num_batched_tokens=max_num_batched_tokens, strategy=scheduling_strategy,
-                          prefill_chunk_size=prefill_chunk_size, enable_cuda_graphs=enable_cuda_graphs)
+                          prefill_chunk_size=prefill_chunk_size, enable_cuda_graphs=enable_cuda_graphs,
+                          kv_cache_dtype=kv_cache_dtype)
     return engine.make_scheduler(eos_token_id=eos_token_id)
 
 
@@ -112,12 +115,15 @@ def main(argv=None) -> int:
     parser.add_argument("--decode-attention-backend", choices=SUPPORTED_DECODE_ATTENTION_BACKENDS, default="cuda",
                         help="single-token decode attention implementation (this engine has one: cuda)")
     parser.add_argument("--kv-cache-dtype", choices=SUPPORTED_KV_CACHE_DTYPES, default="model",
-                        help="KV storage dtype; int8 is not built and is refused")
+                        help="KV storage dtype: the execution dtype, or 4 bits a number; int8 is not built and is refused")
     parser.add_argument("--disable-cuda-graphs", action="store_true",
                         help="disable steady-state decode CUDA-graph replay")
     parser.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
     parser.add_argument("--seed", type=int, default=0, help="seed of random weights and of sampling")
     parser.add_argument("--max-new-tokens", type=int, default=8)
+    parser.add_argument("--score", action="store_true",
+                        help="print the log probabilities of the prompts' tokens instead of generating")
+    parser.add_argument("--top-logprobs", type=int, default=0, help="with --score: most likely tokens to print at each place")
     parser.add_argument("--prompt-ids", action="append",
                         help="a prompt as token ids, e.g. '5 17 3' (may be given several times)")
     parser.add_argument("--prompt-file", help="file with one prompt of token ids per line")
@@ -139,6 +145,13 @@ def main(argv=None) -> int:
         # the reference's demo submits two prompts with max_new_tokens=8 (main.py:337-342)
         vocab = scheduler.engine.vocab_size
         prompts = [[(7 * i + 3) % vocab for i in range(5)], [(11 * i + 1) % vocab for i in range(3)]]
+    if args.score:
+        for index, result in enumerate(scheduler.engine.score(prompts, top=args.top_logprobs)):
+            print(f"prompt {index}: {result.total:.6f} over {len(result.logprobs)} tokens")
+            for place, (logprob, entropy) in enumerate(zip(result.logprobs, result.entropies)):
+                best = "".join(f" {token}:{value:.6f}" for token, value in result.alternatives[place])
+                print(f"  {prompts[index][place + 1]} {logprob:.6f} entropy {entropy:.6f}{best and ' top' + best}")
+        return 0
     ids = [scheduler.add_token_request(prompt, max_new_tokens=args.max_new_tokens,
                                        temperature=args.temperature, seed=args.seed + index)
            for index, prompt in enumerate(prompts)]

@@ -114,7 +114,8 @@ class Model:
 
     # ------------------------------------------------------------------ forward
     def forward(self, ctx) -> torch.Tensor:
-        """Run the tokens of ``ctx`` from the cache; return float32 logits ``[R, V]``."""
+        """Run the tokens of ``ctx`` from the cache; return float32 logits ``[R, V]`` (or, where the step scores given
+        tokens, what the head says about them)."""
         cache = ctx.cache
         if self.embedding.state_need() is not None:
             hidden = self.embedding.forward(ctx, self.positions, state=cache.state.get(self.spec.num_cache_layers))
@@ -151,6 +152,9 @@ class Model:
         hidden = self.blocks[schedule[-1].layer].end(hidden, ctx)
         if arena is not None:
             arena.release(mark)
+        if ctx.scoring is not None:
+            targets, top = ctx.scoring
+            return self.head.score(self.final_norm.forward(hidden, rows=ctx.logit_rows), self.embedding, targets, top)
         if ctx.num_logit_rows == 0:
             return torch.empty((0, self.spec.vocab_size), dtype=torch.float32, device=hidden.device)
         if hasattr(self.final_norm, "defer"):

@@ -31,6 +31,7 @@ class CausalSelfAttention(Mixer):
 
     graph_safe = True
     accepts_deferred_norm = True       # x goes straight into ops.linear_qkv
+    packs_cache = True
 
     def __init__(self, params, prefix, env):
         super().__init__(params, prefix, env)
@@ -206,6 +207,10 @@ class RotaryAttention(Mixer):
     def cache_need(self):
         p = self.params
         return KVNeed(p["n_kv_heads"], self.slot_dim, p.get("window"), chunk=p.get("chunk"))
+
+    @property
+    def packs_cache(self):
+        return self.talk_name is None          # (mixed heads meet every head's values)
 
     def state_need(self):
         if self.conv is None or self.conv["taps"] < 2:

@@ -162,6 +162,10 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    # Whether the mixer's keys and values may be held in 4 bits: it writes and reads them through ``ops.attention``,
+    # ``ops.linear_qkv`` and the rotary cache writes alone, in two planes.
+    packs_cache = False
+
     # What ``forward`` adds is the mixer's result divided by this common factor (1 for nearly all of them): a block that
     # norms the result multiplies by it first (``Block.takes_output_scale``), other blocks refuse such a mixer.
     output_scale = 1.0
@@ -237,6 +241,10 @@ class Head(Part):
 
     def forward(self, x_rows: torch.Tensor, embedding: Embedding) -> torch.Tensor:
         raise NotImplementedError
+
+    def score(self, x_rows: torch.Tensor, embedding: Embedding, targets: torch.Tensor, top: int):
+        """What the logits say about one token a row (``ops.token_logprobs``), for callers that want no logits."""
+        return self.env.ops.token_logprobs(self.forward(x_rows, embedding), targets, top)
 
 
 # ---------------------------------------------------------------------------- registry

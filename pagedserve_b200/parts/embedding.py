@@ -144,3 +144,6 @@ class LMHead(Head):
         if x_rows.shape[0] == 0:
             return logits
         return self.env.ops.linear(x_rows, table, None, logits)
+
+    def score(self, x_rows, embedding, targets, top):
+        return self.env.ops.head_logprobs(x_rows, embedding.table if self.table is None else self.table, targets, top)

@@ -54,6 +54,10 @@ class ParallelMixers(Mixer):
         # (a scale of zero takes its mixer out: its columns of the output matrix become zeros)
         self.output_scale = fixed[0] if fixed and fixed[0] != 0.0 else 1.0
 
+    @property
+    def packs_cache(self):
+        return all(member.packs_cache for member in self.members if member.cache_need() is not None)
+
     def cache_need(self):
         return next((need for need in (member.cache_need() for member in self.members) if need is not None), None)
 
