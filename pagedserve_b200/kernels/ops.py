@@ -137,6 +137,7 @@ _SIGNATURES = {
         "ps_kv_append_packed": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P],
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
+        "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
         "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     },
     "bf16": {
@@ -1289,10 +1290,11 @@ class Ops:
         return rows
 
     def packed_attention_tokens(self, q, out, k_pool, v_pool, page_stride, token_row, positions, block_table, n_heads, n_kv_heads, head_dim,
-                                page_size, window, scale, max_kv_len, softcap=None, sink=None):
+                                page_size, window, scale, max_kv_len, softcap=None, sink=None, shares=0):
         """Attention of single tokens over a packed cache: token t, at ``positions[t]``, reads the pages of row ``token_row[t]`` of
         ``block_table``.  ``max_kv_len`` bounds every token's context (it fixes the grid, so a CUDA graph passes the longest).  ``out`` may be float32
-        in bfloat16.  A token at a position below 0 sees nothing: its row becomes zero.  Otherwise as :meth:`paged_attention_decode`."""
+        in bfloat16.  A token at a position below 0 sees nothing: its row becomes zero.  ``shares``: CTAs for the keys of a token, 1, 2, 4 or 8 (0: by the
+        counts).  Otherwise as :meth:`paged_attention_decode`."""
         what = "packed_attention_tokens"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
@@ -1300,11 +1302,24 @@ class Ops:
         self._indices(what, T, device, token_row=token_row, positions=positions)
         if T == 0:
             return out
-        shares = 1
-        tiles = -(-int(max_kv_len) // 128)
-        while shares < 8 and T * n_heads * shares * 2 <= 2 * 148 * 8 and shares * 2 <= tiles:
-            shares *= 2
+        extent = abs(window or 0)                                     # (a chunked mask, negative, bounds the keys alike)
+        keys = min(int(max_kv_len), extent) if extent else int(max_kv_len)
         self.launches += 1
+        if self.dtype == torch.bfloat16 and head_dim <= 128:
+            if not shares:
+                ctas, most = T * n_kv_heads * -(-n_heads // n_kv_heads // 16), keys // 128
+                shares = 1
+                while shares < 8 and ctas * shares * 2 <= 1184 and shares * 2 <= most:
+                    shares *= 2
+            _check(self._packed_library().ps_packed_tokens_mma(
+                _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
+                page_stride, _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim,
+                page_size, window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, _stream()), what)
+            return out
+        if not shares:
+            shares, most = 1, keys // 128
+            while shares < 8 and T * n_heads * shares * 2 <= 2 * 148 * 8 and shares * 2 <= most:
+                shares *= 2
         _check(self._packed_library().ps_packed_tokens_simt(
             _ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(out.dtype), _ptr(k_pool), _ptr(v_pool), n_pages, page_stride,
             _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim, page_size,
