@@ -138,6 +138,8 @@ _SIGNATURES = {
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
+        "ps_head_logprobs_strips": [_I, _I],
+        "ps_head_logprobs": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P],
         "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     },
     "bf16": {
@@ -2314,11 +2316,42 @@ class Ops:
                                            _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), what)
         return results
 
+    FUSED_HEAD_ROWS, FUSED_HEAD_VOCABULARY, FUSED_HEAD_MOST, SAMPLED = 96, 8192, 4096, 2048
+
+    def fused_head_ok(self, x, table):
+        """Whether the log probabilities of these rows are read inside the head's product: many rows of a large vocabulary in bfloat16."""
+        return (self.dtype == torch.bfloat16 and x.shape[0] >= self.FUSED_HEAD_ROWS and table.shape[0] >= self.FUSED_HEAD_VOCABULARY
+                and self.tc_ok(x, table))
+
+    def _fused_head(self, x, table, targets, top, status, results):
+        (rows, K), V, device = x.shape, table.shape[0], x.device
+        library = self._packed_library()
+        strips = library.ps_head_logprobs_strips(rows, V)
+        sums, given = self.empty((rows, 4 * strips, 3), torch.float32, device), self.empty((rows,), torch.float32, device)
+        sample = entries = count = limit = limit_index = None
+        every, n = 1, V
+        if top:
+            every = -(-V // self.SAMPLED)
+            n = -(-V // every)
+            sample = self.empty((rows, -(-n // 4) * 4), torch.float32, device)
+            if rows > 1024:                              # (2,047 x 2,011 x 768: 10 us in tiles 256 wide, 17 in 128)
+                self.linear_tc(x, table[::every], None, sample[:, :n], bn=256)
+            else:
+                self.linear(x, table[::every], None, sample[:, :n])
+            entries = self.empty((rows, 2048), torch.int64, device)
+            count, limit_index = self.empty((rows,), torch.int32, device), self.empty((rows,), torch.int32, device)
+            limit = self.empty((rows,), torch.float32, device)
+        self.launches += 3 if top else 2
+        _check(library.ps_head_logprobs(
+            _ptr(x), x.stride(0), _ptr(table), table.stride(0), rows, V, K, _ptr(targets), top, _ptr(sample), sample.stride(0) if top else 0, n, every,
+            _ptr(sums), _ptr(given), _ptr(entries), _ptr(count), _ptr(limit), _ptr(limit_index), strips, _ptr(results.logprob),
+            _ptr(results.entropy), _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), "head_logprobs")
+
     LOGITS_AT_ONCE = 1 << 24          # logits that stay in L2 between the product and what is read from them
 
     def head_logprobs(self, x, table, targets, top=0, status=None):
-        """:meth:`token_logprobs` of the logits ``x @ table.T`` (operands of the compute type, logits in float32), some rows at a time: all
-        logits at once never exist."""
+        """:meth:`token_logprobs` of the logits ``x @ table.T`` (operands of the compute type, logits in float32): formed and read some rows at a time,
+        or, where there are many in bfloat16, read inside the product (csrc/head_logprobs.cu); all logits at once never exist."""
         what = "head_logprobs"
         if hasattr(x, "materialize"):
             x = x.materialize()
@@ -2330,8 +2363,16 @@ class Ops:
             raise KernelError(f"{what}: x and table must be rows on one device")
         rows, V = x.shape[0], table.shape[0]
         results = self._logprob_results(what, rows, V, targets, top, x.device)
+        if status is None:
+            status = self.status_flag(x.device)
+        if self.fused_head_ok(x, table):
+            for start in range(0, rows, self.FUSED_HEAD_MOST):
+                part = slice(start, min(rows, start + self.FUSED_HEAD_MOST))
+                self._fused_head(x[part], table, targets[part], top, status, TokenLogprobs(*(result[part] for result in results)))
+            return results
         at_once = max(128, self.LOGITS_AT_ONCE // V // 128 * 128)
-        logits = self.empty((min(rows, at_once), V), torch.float32, x.device)
+        # (rows of whole 16-byte pieces: the product stores them by TMA)
+        logits = self.empty((min(rows, at_once), -(-V // 4) * 4), torch.float32, x.device)[:, :V]
         for start in range(0, rows, at_once):
             end = min(rows, start + at_once)
             part = logits[:end - start]

@@ -100,6 +100,36 @@ def test_from_the_heads_rows(dtype, rows, width, V, top):
     check(ops.head_logprobs(x, table, targets, top), logits, targets, top)
 
 
+@pytest.mark.parametrize("kind", ["zero rows", "rising", "every other sampled", "one token", "infinite"])
+@pytest.mark.parametrize("rows", [96, 300])
+def test_heads_that_fool_a_sample(kind, rows):
+    """Rows whose logits are all equal, rise with the token, or are least at every token that a regular sample meets; a table with a row that is not finite."""
+    ops, width, V, top = ops_for(torch.bfloat16), 64, 20000, 20
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = ((torch.randn(rows, width, generator=g, device=DEV) * 8).round() / 8).clamp(-6, 6)
+    table = ((torch.randn(V, width, generator=g, device=DEV) * 20).round() / 512).clamp(-0.49, 0.49)
+    i = torch.arange(V, device=DEV)
+    if kind == "zero rows":
+        x[::3] = 0
+    elif kind == "rising":
+        table[:, 0], x[:, 0] = (i // 100 * 0.25), 1.0                   # (multiples of 1/4 up to 50: exact in bfloat16)
+    elif kind == "every other sampled":
+        table[:, 0], x[:, 0] = torch.where(i % (V // 2048) == 0, -8.0, 8.0), 4.0
+    elif kind == "one token":
+        table[V - 1, 0], x[:, 0] = 16.0, 4.0
+    x, table = x.bfloat16(), table.bfloat16()
+    if kind == "infinite":
+        table[777, 5] = float("inf")
+        x[:, 5] = torch.where(torch.arange(rows, device=DEV) % 2 == 0, -1.0, 1.0).bfloat16()       # minus infinity in even rows, infinity in odd ones
+    targets = torch.randint(V, (rows,), generator=g, device=DEV).int()
+    found = ops.head_logprobs(x, table, targets, top)
+    logits = x.double() @ table.double().t()
+    if kind == "infinite":
+        assert found.logprob[1::2].isnan().all() and found.entropy[1::2].isnan().all() and (found.top_ids[1::2, 0] == 777).all()
+        found, logits, targets = type(found)(*(t[::2] for t in found)), logits[::2], targets[::2]
+    check(found, logits, targets, top)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_captured_head(dtype):
     """Captured on a side stream and replayed with other rows."""
