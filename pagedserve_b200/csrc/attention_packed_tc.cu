@@ -1,0 +1,676 @@
+// Causal attention of prompt portions over a cache held in 4 bits on tcgen05 tensor cores (bfloat16 queries, head sizes up to 128; packed.cuh
+// has the cache's format).
+//
+// One CTA per (block of 256 query tokens of one request, head), tiles of 128 keys aligned to absolute positions. The block is two tiles of 128
+// queries that take turns: while the rows of one form their weights, the tensor cores work for the other.
+//   warps 0..3   a key a thread: its codes and scales come to registers a tile ahead, become low + code * step (one rounding to float16, 2^-12 of
+//                the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact as its own)
+//                and go to the swizzled tile, 16 bytes a word of codes; before that the second query tile's rows
+//   warps 4..7   the same of the values and the first query tile
+//   warps 8, 17  issue of S = Q K^T and O += P V for the first and the second query tile (8: TMEM allocation, too)
+//   warps 9..16  softmax, a thread per query row: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves, and O with it, only when
+//                a score is beyond it by 2^8, which float16 has room for
+// A tile's keys go through in two halves of 64, whose scores have columns of their own: P of a half takes the place of its scores, P V of the half is
+// issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half. Rows hardly wait, then.
+// Queries are scaled row by row by a power of two, so that any bfloat16 row is one in float16. Keys and values are not: a block that meets one
+// beyond 60,000, or none beyond 2^-9, or a NaN, or a key without a page, forms its rows again in float32 from the codes (rows_again below), which is slow and
+// right.
+//
+// What bounds it: exponentials, 16 a clock and SM: 2,048 clocks for 256 queries and 128 keys, as long as the products at head size 128.  One tile's scores at a time
+// for a query tile (scores, weights, P V, scores in turn) took 4,700 clocks at head size 64, 2,200 of them the way from P to the next scores; an MMA takes about 70 clocks
+// to issue, so either query tile has a warp for it.
+#include <type_traits>
+
+#include "packed.cuh"
+
+namespace ps {
+namespace packedtc {
+
+using namespace packed;
+
+constexpr int BQ = 128, BKEY = 128, MAKERS = 128, THREADS = 2 * MAKERS + 64 + 2 * BQ;                  // MAKERS: of keys, and of values
+constexpr uint64_t WAIT_LIMIT_NS = 200ull * 1000 * 1000;
+constexpr float MOST = 60000.f, LEAST = 0.001953125f;              // sizes of numbers that float16 holds to 2^-12 of the largest
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t timer_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+// false: the wait ran out, or another role of this CTA gave up
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    // (the timer is read only after many tries: a read takes longer than most waits)
+#pragma unroll 1
+    for (int spin = 0; spin < 2048; ++spin)
+        if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t start = timer_ns();
+    while (true) {
+#pragma unroll 1
+        for (int spin = 0; spin < 64; ++spin)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (timer_ns() - start > WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
+    }
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo_bytes) {
+    uint64_t desc = (uint64_t)((smem_addr >> 4) & 0x3FFF);
+    desc |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
+    desc |= (uint64_t)(1024 >> 4) << 32;
+    desc |= (uint64_t)1 << 46;
+    desc |= (uint64_t)2 << 61;
+    return desc;
+}
+// Issued by the thread of a warp whose `one` is set, while the whole warp comes along: its control flow and descriptors then stay uniform. (Inside a branch
+// that one lane takes, an MMA's operands are moved to uniform registers one by one: 80 clocks an MMA, 960 for a tile's twelve.)
+__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(one) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t half_add(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t half_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// the byte of a tile ([HD / 64][128 rows][128 bytes], swizzled) at which the eight numbers from d on of a row stand
+__device__ __forceinline__ uint32_t tile_byte(int row, int d) {
+    return (uint32_t)((d >> 6) * (128 * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4));
+}
+// a word of codes as eight float16 numbers low + code * step
+__device__ __forceinline__ uint4 numbers_of(uint32_t word, uint32_t step, uint32_t low) {
+    const uint32_t next = word >> 8;
+    uint4 v;                                                       // codes 1024 + c and 64 + c, less those: whole numbers, exactly
+    v.x = half_fma(half_add((word & 0x000f000fu) | 0x64006400u, 0xe400e400u), step, low);
+    v.y = half_fma(half_add((word & 0x00f000f0u) | 0x54005400u, 0xd400d400u), step, low);
+    v.z = half_fma(half_add((next & 0x000f000fu) | 0x64006400u, 0xe400e400u), step, low);
+    v.w = half_fma(half_add((next & 0x00f000f0u) | 0x54005400u, 0xd400d400u), step, low);
+    return v;
+}
+
+template <int HD>
+struct Layout {
+    static constexpr int KV_STAGES = 2, KCH = HD / 64, Q_BYTES = BQ * HD * 2, KV_BYTES = BKEY * HD * 2, STAGE_BYTES = 2 * KV_BYTES;
+    // two query tiles, the stages, barriers (256 bytes), the rows' factors, then a few words
+    static constexpr size_t SMEM = 2 * Q_BYTES + (size_t)KV_STAGES * STAGE_BYTES + 1024 + 256 + 2 * BQ * 4 + 16;
+    // TMEM: scores of either tile (P takes their place), then O of either
+    static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
+};
+constexpr float HEADROOM = 8.f;                                     // log2 of how far a weight may be beyond 1 before its base moves
+
+struct Cache {
+    const unsigned char* k_pool;
+    const unsigned char* v_pool;
+    long long page_stride;
+    Pages pages;
+};
+
+// Rows of a block once more, in float32 from the codes, a warp a row: lane l has number 32 j + l of every group.
+__device__ __noinline__ void rows_again(const __nv_bfloat16* q, long long q_stride, void* out, long long out_stride, int wide, const Cache cache, int table_row,
+                                        long long head_at, int h, int head_dim, int tok0, int pos0, int rows, int window, float scale,
+                                        float softcap, const float* sink, int warp, int warps, int lane) {
+    const int groups = groups_of(head_dim), page_size = 1 << cache.pages.page_log2, shift = code_shift(lane & 7);
+    for (int r = warp; r < rows; r += warps) {
+        const int p = pos0 + r, last = min(p, (cache.pages.bt_stride << cache.pages.page_log2) - 1);
+        float x[4], acc[4], m = -INFINITY, l = 0.f;
+        if (sink) {
+            m = sink[h];
+            l = 1.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = j * GROUP + lane;
+            x[j] = d < head_dim ? __bfloat162float(q[(long long)(tok0 + r) * q_stride + (long long)h * head_dim + d]) : 0.f;
+            acc[j] = 0.f;
+        }
+        for (int key = first_visible_key(p, window); key <= last; ++key) {
+            const int page = cache.pages.of(table_row, key);
+            if (page < 0) continue;
+            const long long at = (long long)page * cache.page_stride + head_at;
+            const int row = key & (page_size - 1);
+            float s = 0.f, v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = 0.f;
+                if (j < groups) {
+                    const int word = (row * 4 + (lane >> 3)) * groups + j, scale_at = page_size * groups * 4 + row * groups + j;
+                    const uint32_t *k = reinterpret_cast<const uint32_t*>(cache.k_pool + at), *w = reinterpret_cast<const uint32_t*>(cache.v_pool + at);
+                    const bool there = j * GROUP + lane < head_dim;            // (a number that is not there has no code)
+                    if (there) s = fmaf(fmaf((float)(k[word] >> shift & 15u), step_of(k[scale_at]), low_of(k[scale_at])), x[j], s);
+                    v[j] = fmaf((float)(w[word] >> shift & 15u), step_of(w[scale_at]), low_of(w[scale_at]));
+                }
+            }
+            s = warp_sum(s) * scale;
+            if (softcap > 0.f) s = softcap * tanhf(s / softcap);
+            const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, shrink = expf(m - base), w = expf(s - base);
+            m = top;
+            l = fmaf(l, shrink, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = fmaf(acc[j], shrink, w * v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = j * GROUP + lane;
+            const float result = l == 0.f ? acc[j] * 0.f : acc[j] / l;
+            const long long to = (long long)(tok0 + r) * out_stride + (long long)h * head_dim + d;
+            if (d < head_dim) {
+                if (wide) reinterpret_cast<float*>(out)[to] = result;
+                else reinterpret_cast<__nv_bfloat16*>(out)[to] = __float2bfloat16_rn(result);
+            }
+        }
+    }
+}
+
+template <int HD, bool CAPPED>
+__global__ void __launch_bounds__(THREADS, 1)
+prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __restrict__ out, long long out_stride, Cache cache,
+               const int* __restrict__ q_start, const int* __restrict__ kv_len, const int* __restrict__ item_row, int n_items, int n_heads,
+               int n_kv_heads, int head_dim, int window, float scale, float softcap, SoftmaxExtras extras, int aligned_q, int aligned_out,
+               int* __restrict__ status) {
+    using L = Layout<HD>;
+    constexpr int KV_STAGES = L::KV_STAGES, GROUPS_MOST = HD / GROUP;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* q_s = base;                // two tiles
+    unsigned char* kv_s = base + 2 * L::Q_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + (size_t)KV_STAGES * L::STAGE_BYTES);
+    uint64_t* q_full = bars;                  // [2] makers -> MMA and rows
+    uint64_t* k_full = q_full + 2;            // [KV_STAGES] makers -> MMA
+    uint64_t* k_empty = k_full + KV_STAGES;   // [KV_STAGES] MMA -> makers
+    uint64_t* v_full = k_empty + KV_STAGES;   // [KV_STAGES] makers -> MMA
+    uint64_t* v_empty = v_full + KV_STAGES;   // [KV_STAGES] MMA -> makers
+    uint64_t* s_full = v_empty + KV_STAGES;   // [2 query tiles][2 halves] MMA -> rows: the half's scores are complete
+    uint64_t* p_ready = s_full + 4;           // [2][2] rows -> MMA: P of the half is in TMEM, O is in its units
+    uint64_t* o_done = p_ready + 4;           // [2] MMA -> rows: P V of a half is complete
+    uint64_t* o_full = o_done + 2;            // [2] MMA -> rows: O is complete (o_done could be a phase or two behind where no one waited for it)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* factor_s = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(bars) + 256);      // [2 * BQ] what undoes a query row's scale
+    uint32_t* sizes_s = reinterpret_cast<uint32_t*>(factor_s + 2 * BQ);          // largest key, largest value (bits), whether something is strange
+
+    pdl_prologue();
+    q = pdl_fresh(q);
+    cache.k_pool = pdl_fresh(cache.k_pool);
+    cache.v_pool = pdl_fresh(cache.v_pool);
+    int block = blockIdx.y, item = -1, qb = 0;                    // late blocks see most keys: they come first
+    for (int i = 0; i < n_items; ++i) {
+        const int blocks = (q_start[i + 1] - q_start[i] + 2 * BQ - 1) / (2 * BQ);
+        if (block < blocks) { item = i; qb = blocks - 1 - block; break; }
+        block -= blocks;
+    }
+    if (item < 0) return;
+    const int h = blockIdx.x, g = h / (n_heads / n_kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int qs = q_start[item], q_len = q_start[item + 1] - qs;
+    const int pos0 = kv_len[item] - q_len + qb * 2 * BQ;              // position of the block's first query
+    const int rows = min(2 * BQ, q_len - qb * 2 * BQ), tok0 = qs + qb * 2 * BQ;
+    const int hi = pos0 + rows - 1, lo = pos0 < 0 ? 0 : first_visible_key(pos0, window);
+    const int kb_first = lo / BKEY, kb_last = max(hi, 0) / BKEY;
+    // the key tiles that a query tile's rows see (a second tile without rows: none)
+    auto first_of = [&](int x) {
+        const int p = pos0 + x * BQ;
+        return x * BQ >= rows ? kb_last + 1 : (p < 0 ? 0 : first_visible_key(p, window)) / BKEY;
+    };
+    auto last_of = [&](int x) { return max(pos0 + min(rows, (x + 1) * BQ) - 1, 0) / BKEY; };
+    const int table_row = item_row ? item_row[item] : item;
+    const int page_size = 1 << cache.pages.page_log2, groups = groups_of(head_dim);
+    const long long head_at = (long long)g * slab_bytes(page_size, head_dim);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < KV_STAGES; ++s) {
+            mbar_init(&k_full[s], MAKERS); mbar_init(&k_empty[s], 2);
+            mbar_init(&v_full[s], MAKERS); mbar_init(&v_empty[s], 2);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&q_full[x], MAKERS);
+            for (int half = 0; half < 2; ++half) {
+                mbar_init(&s_full[2 * x + half], 1);
+                mbar_init(&p_ready[2 * x + half], BQ);
+            }
+            mbar_init(&o_done[x], 1);
+            mbar_init(&o_full[x], 1);
+        }
+        sizes_s[0] = sizes_s[1] = sizes_s[2] = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)L::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp < 8) {
+        // ------------------------------------------------ makers: thread r has key r of every tile, and row r of the second query tile, or the value and
+        // row of the first
+        const int r = threadIdx.x & 127;
+        const bool values = warp >= 4;
+        const unsigned char* pool = (values ? cache.v_pool : cache.k_pool) + head_at;
+        uint4 codes[GROUPS_MOST], next_codes[GROUPS_MOST];
+        uint32_t scales[GROUPS_MOST], next_scales[GROUPS_MOST];
+        bool strange = false;
+        float most_size = 0.f;
+        auto fetch = [&](int kb) {
+            const int key = kb * BKEY + r;
+            const bool needed = key >= lo && key <= hi;
+            const int page = needed ? cache.pages.of(table_row, key) : -1;
+            strange |= needed && page < 0;
+            const int row = key & (page_size - 1);
+            const unsigned char* at = pool + (long long)page * cache.page_stride;
+#pragma unroll
+            for (int j = 0; j < GROUPS_MOST; ++j) {
+                const bool there = page >= 0 && j < groups;
+                next_codes[j] = there ? *reinterpret_cast<const uint4*>(at + (row * groups + j) * 16) : make_uint4(0, 0, 0, 0);
+                next_scales[j] = there ? *reinterpret_cast<const uint32_t*>(at + page_size * groups * 16 + (row * groups + j) * 4) : 0u;
+            }
+        };
+        auto take = [&]() {
+#pragma unroll
+            for (int j = 0; j < GROUPS_MOST; ++j) {
+                codes[j] = next_codes[j];
+                scales[j] = next_scales[j];
+            }
+        };
+        // a row of a tile: place p of the codes (part p / groups of group p % groups) becomes eight numbers; what is not there becomes zeros
+        auto make = [&](unsigned char* tile) {
+            uint32_t step[GROUPS_MOST], low[GROUPS_MOST];
+#pragma unroll
+            for (int j = 0; j < GROUPS_MOST; ++j) {
+                const float a = step_of(scales[j]), b = low_of(scales[j]), size = fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b)));
+                strange |= !(size <= MOST);
+                most_size = fmaxf(most_size, size);
+                step[j] = half_pair(a, a);
+                low[j] = half_pair(b, b);
+            }
+            auto put = [&](auto count) {
+                constexpr int NG = decltype(count)::value;
+#pragma unroll
+                for (int p = 0; p < 4 * NG; ++p) {
+                    const uint4& four = codes[p >> 2];
+                    const uint32_t word = (p & 3) == 0 ? four.x : (p & 3) == 1 ? four.y : (p & 3) == 2 ? four.z : four.w;
+                    *reinterpret_cast<uint4*>(tile + tile_byte(r, (p % NG) * GROUP + p / NG * 8)) = numbers_of(word, step[p % NG], low[p % NG]);
+                }
+#pragma unroll
+                for (int d = NG * GROUP; d < HD; d += 8) *reinterpret_cast<uint4*>(tile + tile_byte(r, d)) = make_uint4(0, 0, 0, 0);
+            };
+            if constexpr (GROUPS_MOST == 2) {
+                if (groups == 2) put(std::integral_constant<int, 2>());
+                else put(std::integral_constant<int, 1>());
+            } else {
+                if (groups == 4) put(std::integral_constant<int, 4>());
+                else put(std::integral_constant<int, 3>());
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        fetch(kb_first);
+        {
+            const int x = values ? 0 : 1, place = x * BQ + r;
+            const __nv_bfloat16* row = q + (long long)(tok0 + place) * q_stride + (long long)h * head_dim;
+            float most = 0.f;
+            bool odd = false;
+            // twice over the row: for its largest number, and for its numbers (its 128 or 256 bytes stay in L1)
+            auto load = [&](int d, float (&n)[8]) {
+                if (place < rows && aligned_q && d < head_dim) {
+                    const uint4 raw = *reinterpret_cast<const uint4*>(row + d);
+                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        n[2 * i] = __uint_as_float(w[i] << 16);
+                        n[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) n[i] = place < rows && d + i < head_dim ? __bfloat162float(row[d + i]) : 0.f;
+                }
+            };
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float n[8];
+                load(d, n);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    most = fmaxf(most, fabsf(n[i]));
+                    odd |= !(fabsf(n[i]) <= 3.4028235e38f);
+                }
+            }
+            // 2^up brings the largest to [256, 512); a NaN or infinity stays one
+            const int up = most > 0.f && !odd ? min(126, 135 - max(1, (int)(__float_as_uint(most) >> 23))) : 0;
+            const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+            factor_s[place] = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float n[8];
+                load(d, n);
+                uint4 v;
+                v.x = half_pair(n[0] * by, n[1] * by);
+                v.y = half_pair(n[2] * by, n[3] * by);
+                v.z = half_pair(n[4] * by, n[5] * by);
+                v.w = half_pair(n[6] * by, n[7] * by);
+                *reinterpret_cast<uint4*>(q_s + x * L::Q_BYTES + tile_byte(r, d)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&q_full[x]);
+        }
+        uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+        uint32_t it = 0;
+        for (int kb = kb_first; kb <= kb_last; ++kb, ++it) {
+            const int s = it % KV_STAGES;
+            take();
+            if (kb < kb_last) fetch(kb + 1);
+            if (!mbar_wait(&empty[s], ((it / KV_STAGES) & 1) ^ 1, abort_flag)) { if (lane == 0) atomicExch(status, values ? 52 : 51); break; }
+            make(kv_s + (size_t)s * L::STAGE_BYTES + (values ? L::KV_BYTES : 0));
+            mbar_arrive(&full[s]);
+        }
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most_size));
+        const bool any = __any_sync(0xffffffffu, strange);
+        if (lane == 0) {
+            atomicMax(&sizes_s[values ? 1 : 0], bits);
+            if (any) atomicExch(&sizes_s[2], 1u);
+        }
+    } else if (warp == 8 || warp == 17) {
+        // ------------------------------------------------ MMA issuers, one for each query tile
+        // D f32, A/B f16: S = Q K^T both K-major, N = 64; O = P V with A from TMEM and B MN-major (bit 16), N = HD
+        constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        const uint32_t one = lane == 0 ? 1u : 0u;
+        const int x = warp == 8 ? 0 : 1, first = first_of(x), last = last_of(x);
+        const uint32_t s_at = tmem_base + L::S_COL + x * 128, o_at = tmem_base + L::O_COL + x * HD;
+        const uint64_t q_desc = desc_sw128(smem_u32(q_s + x * L::Q_BYTES), 16);
+        auto waits = [&](uint64_t* bar, uint32_t parity, int code) {
+            const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+            if (!there && lane == 0) atomicExch(status, code);
+            tc_fence_after();
+            return there;
+        };
+        auto scores = [&](int kb, int half) {                      // (64 rows of a tile are 8,192 bytes)
+            const uint64_t k_desc = desc_sw128(smem_u32(kv_s + (size_t)((kb - kb_first) % KV_STAGES) * L::STAGE_BYTES) + half * 8192, 16);
+#pragma unroll
+            for (int c = 0; c < L::KCH; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_ss(one, s_at + half * 64, q_desc + c * (BQ * 128 / 16) + 2 * k, k_desc + c * (BKEY * 128 / 16) + 2 * k, idesc_qk, (c | k) ? 1u : 0u);
+            umma_commit(one, &s_full[2 * x + half]);
+        };
+        bool ok = true;
+        uint32_t taken = 0;                                        // key tiles of this query tile whose weights were taken
+        for (int kb = kb_first - 1; kb <= kb_last && ok; ++kb) {   // weights of tile kb, scores of kb + 1
+            const uint32_t it = (uint32_t)(kb - kb_first);
+            const bool weighs = kb >= first && kb <= last, next = kb + 1 <= kb_last, asks = kb + 1 >= first && kb + 1 <= last;
+            if (next) ok = waits(&k_full[(it + 1) % KV_STAGES], ((it + 1) / KV_STAGES) & 1, 54);
+            if (ok && kb + 1 == first) ok = waits(&q_full[x], 0, 53);
+            if (ok && kb >= kb_first) ok = waits(&v_full[it % KV_STAGES], (it / KV_STAGES) & 1, 57);
+#pragma unroll 1
+            for (int half = 0; half < 2 && ok; ++half) {
+                if (weighs) {
+                    ok = waits(&p_ready[2 * x + half], taken & 1, 56);
+                    if (!ok) break;
+                    const uint64_t v_desc = desc_sw128(smem_u32(kv_s + (size_t)(it % KV_STAGES) * L::STAGE_BYTES) + L::KV_BYTES + half * 8192, BKEY * 128);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)                    // 16 keys = 2,048 bytes of V, 8 columns of P
+                        umma_ts(one, o_at, s_at + half * 64 + 8 * k, v_desc + (uint64_t)((2048 * k) >> 4), idesc_pv, (taken | (uint32_t)half | (uint32_t)k) ? 1u : 0u);
+                    umma_commit(one, &o_done[x]);
+                    if (kb == last && half == 1) umma_commit(one, &o_full[x]);
+                }
+                if (asks) scores(kb + 1, half);
+            }
+            if (ok && weighs) ++taken;
+            // (a tile that this query tile does not see is given back as soon as it is there)
+            if (ok && kb >= kb_first) umma_commit(one, &v_empty[it % KV_STAGES]);
+            if (ok && next) umma_commit(one, &k_empty[(it + 1) % KV_STAGES]);
+        }
+    } else {
+        // ------------------------------------------------ rows
+        const int quarter = warp & 3, x = (warp - 9) >> 2;
+        const int r = quarter * 32 + lane, place = x * BQ + r, pos = pos0 + place;
+        const int first = first_of(x), last = last_of(x);
+        const int lo_row = pos < 0 ? 0 : first_visible_key(pos, window);
+        const int pos_first = pos0 + x * BQ, pos_last = pos0 + min(rows, (x + 1) * BQ) - 1;
+        const int lo_all = pos_last < 0 ? 0 : first_visible_key(pos_last, window);        // the first key that every row of the tile sees
+        const uint32_t s_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::S_COL + x * 128;
+        const uint32_t o_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::O_COL + x * HD;
+        float base_m = 0.f, limit = -INFINITY, l_run = 0.f;        // in log2 units: the base of the weights, what a score may reach
+        if (extras.sink && extras.sink[h] != -INFINITY) {
+            base_m = extras.sink[h] * 1.4426950408889634f;
+            limit = base_m + HEADROOM;
+            l_run = 1.f;
+        }
+        bool ok = first <= last && mbar_wait(&q_full[x], 0, abort_flag);
+        if (!ok && first <= last && lane == 0) atomicExch(status, 58);
+        const float factor = ok ? factor_s[place] : 0.f;
+        // (not 0: minus infinity times it is to stay that)
+        const float unit_scale = CAPPED ? 1.0f : fmaxf(scale * 1.4426950408889634f * factor, 1e-37f);
+        const unsigned long long unit2 = pair_of(unit_scale, unit_scale);
+        uint32_t n = 0;                                            // halves so far
+        for (; first * 2 + (int)n < 2 * (last + 1) && ok; ++n) {
+            const int half = n & 1, key0 = first * BKEY + (int)n * 64;
+            if (!mbar_wait(&s_full[2 * x + half], (n >> 1) & 1, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 59); break; }
+            tc_fence_after();
+            uint32_t sr[64];
+            tmem_ld32(s_at + half * 64, sr);
+            tmem_ld32(s_at + half * 64 + 32, sr + 32);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if constexpr (CAPPED) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) sr[j] = __float_as_uint(cap_special(__uint_as_float(sr[j]) * factor, extras));
+            }
+            if (key0 + 63 > pos_first || key0 < lo_all || (x + 1) * BQ > rows) {
+                const int first_ok = place < rows ? lo_row - key0 : 64, last_ok = place < rows ? pos - key0 : -1;
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                    if (j < first_ok || j > last_ok) sr[j] = 0xff800000u;        // -inf
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(sr[j]), __uint_as_float(sr[j + 1]));
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * unit_scale;
+            if (__any_sync(0xffffffffu, top > limit)) {
+                const bool has = limit > -INFINITY, moves = top > limit;
+                const float fresh = moves ? (has ? fmaxf(top, base_m) : top) : base_m, corr = !moves ? 1.f : (has ? ex2(base_m - fresh) : 0.f);
+                base_m = fresh;
+                if (moves) limit = fresh + HEADROOM;
+                l_run *= corr;
+                if (n > 0) {                                       // no P V may be under way: that of the half before has to be done (that of the one before it is: this half's scores followed it)
+                    if (!mbar_wait(&o_done[x], (n - 1) & 1, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 60); break; }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t orr[16];
+                        tmem_ld16(o_at + c, orr);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) orr[j] = __float_as_uint(__uint_as_float(orr[j]) * corr);
+                        tmem_st16(o_at + c, orr);
+                    }
+                }
+            }
+            // weights 2^(s - base)
+            const unsigned long long less = pair_of(-base_m, -base_m);
+            unsigned long long sum_a = 0ull, sum_b = 0ull;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t pr[16];
+#pragma unroll
+                for (int j = c; j < c + 32; j += 4) {
+                    float p[4];
+                    pair_split(pair_fma(pair_of(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])), unit2, less), p[0], p[1]);
+                    pair_split(pair_fma(pair_of(__uint_as_float(sr[j + 2]), __uint_as_float(sr[j + 3])), unit2, less), p[2], p[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = ex2(p[i]);
+                    sum_a = pair_add(sum_a, pair_of(p[0], p[1]));
+                    sum_b = pair_add(sum_b, pair_of(p[2], p[3]));
+                    pr[(j - c) >> 1] = half_pair(p[0], p[1]);
+                    pr[((j - c) >> 1) + 1] = half_pair(p[2], p[3]);
+                }
+                tmem_st16(s_at + half * 64 + (c >> 1), pr);
+            }
+            float even, odd;
+            pair_split(pair_add(sum_a, sum_b), even, odd);
+            l_run += even + odd;
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            mbar_arrive(&p_ready[2 * x + half]);
+        }
+        if (ok && !mbar_wait(&o_full[x], 0, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 61); }
+        if (ok) {
+            tc_fence_after();
+            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+            const long long to = (long long)(tok0 + place) * out_stride + (long long)h * head_dim;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t orr[16];
+                tmem_ld16(o_at + c, orr);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (place < rows) {
+#pragma unroll
+                    for (int d = 0; d < 16; d += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(orr[d + i]) * inv;
+                        if (aligned_out && c + d + 8 <= head_dim) {
+                            if (extras.wide) {
+                                float4* at = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to + c + d);
+                                at[0] = make_float4(v[0], v[1], v[2], v[3]);
+                                at[1] = make_float4(v[4], v[5], v[6], v[7]);
+                            } else {
+                                uint4 pack;
+                                uint32_t* two = reinterpret_cast<uint32_t*>(&pack);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                                    two[i] = *reinterpret_cast<const uint32_t*>(&b);
+                                }
+                                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + to + c + d) = pack;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (c + d + i < head_dim) store_result(reinterpret_cast<__nv_bfloat16*>(out), to + c + d + i, v[i], extras);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)L::TMEM_COLS) : "memory");
+    }
+    const float k_most = __uint_as_float(sizes_s[0]), v_most = __uint_as_float(sizes_s[1]);
+    if (sizes_s[2] || (k_most > 0.f && k_most < LEAST) || (v_most > 0.f && v_most < LEAST))
+        rows_again(q, q_stride, out, out_stride, extras.wide, cache, table_row, head_at, h, head_dim, tok0, pos0, rows, window, scale, softcap, extras.sink,
+                   warp, THREADS / 32, lane);
+}
+
+template <int HD, bool CAPPED>
+int launch(const void* q, long long q_stride, void* out, long long out_stride, int wide, const Cache& cache, const int* q_start, const int* kv_len,
+           const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
+           const float* sink, int* status, cudaStream_t s) {
+    auto kernel = prompts_kernel<HD, CAPPED>;
+    static size_t raised[MAX_DEVICES] = {0};
+    if (!ensure_dynamic_smem((const void*)kernel, Layout<HD>::SMEM, raised)) return PS_ERR_LAUNCH;
+    const int aligned_q = !((uintptr_t)q & 15) && q_stride % 8 == 0 && head_dim % 8 == 0;
+    const int aligned_out = !((uintptr_t)out & 15) && out_stride % 8 == 0 && head_dim % 8 == 0;
+    return launch_pdl(kernel, dim3(n_heads, max_blocks), dim3(THREADS), Layout<HD>::SMEM, s, (const __nv_bfloat16*)q, q_stride, out, out_stride, cache,
+                      q_start, kv_len, item_row, n_items, n_heads, n_kv_heads, head_dim, window, scale, softcap, softmax_extras(scale, softcap, sink, wide),
+                      aligned_q, aligned_out, status);
+}
+
+}  // namespace packedtc
+}  // namespace ps
+
+// q / out: the step's flat rows of n_heads * head_dim numbers; item i's tokens are rows q_start[i] .. q_start[i + 1], the last ones of kv_len[i], its
+// pages row item_row[i] of block_table (bt_stride wide).  max_blocks >= sum over the items of ceil(tokens / 256).  wide: out is float32.
+PS_EXPORT int ps_packed_prompts_tc(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
+                                   int n_pages, long long page_stride, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
+                                   const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int page_size,
+                                   int window, float scale, float softcap, const float* sink, int* status, void* stream) {
+    using namespace ps::packedtc;
+    if (n_items <= 0 || max_blocks <= 0) return PS_OK;
+    if (!q || !out || !k_pool || !v_pool || !q_start || !kv_len || !block_table || !status) return PS_ERR_BAD_ARGUMENT;
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_blocks > 65535) return PS_ERR_BAD_ARGUMENT;
+    if (!ps::packed::sizes_ok(n_kv_heads, head_dim, page_size) || head_dim > 128) return PS_ERR_UNSUPPORTED;
+    if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
+    const Cache cache = {(const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, {block_table, bt_stride, n_pages, ps::packed::log2_of(page_size)}};
+    auto run = head_dim <= 64 ? (softcap > 0.f ? launch<64, true> : launch<64, false>) : (softcap > 0.f ? launch<128, true> : launch<128, false>);
+    return run(q, q_stride, out, out_stride, wide, cache, q_start, kv_len, item_row, n_items, max_blocks, n_heads, n_kv_heads, head_dim, window, scale,
+               softcap, sink, status, (cudaStream_t)stream);
+}

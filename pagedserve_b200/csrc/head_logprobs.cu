@@ -54,7 +54,10 @@ __device__ __forceinline__ uint64_t timer_ns() {
 }
 // false: the wait ran out, or another role of this CTA gave up
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
+    // (the timer is read only after many tries: a read takes longer than most waits)
+#pragma unroll 1
+    for (int spin = 0; spin < 2048; ++spin)
+        if (mbar_try_wait(bar, parity)) return true;
     const uint64_t start = timer_ns();
     while (true) {
 #pragma unroll 1

@@ -36,7 +36,7 @@ LIBRARIES: Dict[str, List[str]] = {
              "rotary.cu", "wkv.cu", "embed_pair.cu", "hyper.cu", "latent.cu", "moe.cu", "post_norm.cu", "mingru.cu",
              "short_conv.cu", "gla.cu", "head_mix.cu", "ssd.cu", "diff_attention.cu"],
     "bf16": ["gemm_skinny.cu", "attention_decode.cu", "attention_prefill.cu", "attention_rows.cu", "attention_lanes.cu"],
-    "packed": ["packed_cache.cu", "attention_packed.cu", "attention_packed_mma.cu", "logprobs.cu", "head_logprobs.cu"],
+    "packed": ["packed_cache.cu", "attention_packed.cu", "attention_packed_mma.cu", "attention_packed_tc.cu", "logprobs.cu", "head_logprobs.cu"],
     "tc": ["gemm_tc.cu", "gemm_rows_tc.cu", "gemm_f32_tc.cu", "attention_prefill_tc.cu", "attention_f32_tc.cu"],
 }
 

@@ -138,6 +138,7 @@ _SIGNATURES = {
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
+        "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P],
         "ps_head_logprobs_strips": [_I, _I],
         "ps_head_logprobs": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P],
         "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
@@ -1277,7 +1278,7 @@ class Ops:
             _ptr(item_row) + 4 * first_item, n_items, span, _ptr(out), out.shape[3], n_kv_heads, head_dim, page_size, self.code, _stream()), what)
         return out
 
-    def _packed_queries(self, what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device):
+    def _packed_queries(self, what, q, out, n_heads, n_kv_heads, head_dim, scale, softcap, sink, device):
         if n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads:
             raise KernelError(f"{what}: n_heads must be a multiple of n_kv_heads")
         rows = q.shape[0]
@@ -1285,6 +1286,8 @@ class Ops:
         self._packed_rows(what, "out", out, rows, n_heads * head_dim, device, (self.dtype, torch.float32))
         if softcap is not None and not softcap > 0:
             raise KernelError(f"{what}: softcap must be positive")
+        if not scale >= 0:
+            raise KernelError(f"{what}: scale cannot be negative")
         if sink is not None and not (sink.dtype is torch.float32 and sink.numel() == n_heads and sink.is_contiguous() and sink.get_device() == device):
             _require(sink, "sink", torch.float32)
             self._on_current_device(what, sink)
@@ -1300,7 +1303,7 @@ class Ops:
         what = "packed_attention_tokens"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
-        T = self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device)
+        T = self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, scale, softcap, sink, device)
         self._indices(what, T, device, token_row=token_row, positions=positions)
         if T == 0:
             return out
@@ -1344,9 +1347,9 @@ class Ops:
         ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  Otherwise as
         :meth:`prefill_attention`."""
         what = "packed_attention_prompts"
-        self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
+        n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
-        self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, softcap, sink, device)
+        self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, scale, softcap, sink, device)
         if first_item < 0 or n_items < 0:
             raise KernelError(f"{what}: items below 0")
         self._indices(what, first_item + n_items, device, kv_len=kv_len, item_row=item_row)
@@ -1356,7 +1359,16 @@ class Ops:
             return out
         if not self.packed_prompts_ok(q, out, head_dim, max_blocks):
             raise KernelError(f"{what}: heads of {head_dim} in {self.dtype} with these strides go token by token (packed_attention_tokens)")
-        # The rows as pages of the compute type, some items at a time, and the kernel for those.
+        if self.dtype == torch.bfloat16:
+            # (an entry of b blocks of 64 queries has at most (b + 3) / 4 of 256)
+            self.launches += 1
+            _check(self._packed_library().ps_packed_prompts_tc(
+                _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
+                page_stride, _ptr(q_start) + 4 * first_item, _ptr(kv_len) + 4 * first_item, _ptr(block_table), block_table.shape[1],
+                _ptr(item_row) + 4 * first_item, n_items, (max_blocks + 3 * n_items) // 4, n_heads, n_kv_heads, head_dim, page_size, window or 0, scale,
+                float(softcap or 0.0), _ptr(sink), _ptr(self.status_flag(device)), _stream()), what)
+            return out
+        # float32: the rows as pages of the compute type, some items at a time, and the kernels for those.
         page = 64
         span = min(-(-int(max_kv_len) // page) * page, -(-block_table.shape[1] * page_size // page) * page)
         item_bytes = span * 2 * n_kv_heads * head_dim * self.dtype.itemsize
@@ -1372,34 +1384,26 @@ class Ops:
         return out
 
     def packed_prompts_ok(self, q, out, head_dim, max_blocks):
-        """Whether :meth:`packed_attention_prompts` takes these rows: float32 heads of up to 128 numbers in whole 16-byte pieces, bfloat16 ones
-        in multiples of 16 up to 128."""
+        """Whether :meth:`packed_attention_prompts` takes these rows: heads of up to 128 numbers, in float32 in whole 16-byte pieces."""
         if self.dtype == torch.float32:
             return (head_dim % 4 == 0 and head_dim <= 128 and max_blocks <= 65535 and q.stride(0) % 4 == 0 and out.stride(0) % 4 == 0
                     and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
-        return head_dim % 16 == 0 and head_dim <= 128 and max_blocks <= 65535 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+        return head_dim <= 128 and max_blocks <= 65535
 
     def _prompts_from_pages(self, q, out, pool, q_start, kv_len, table, item_row, n_items, max_blocks, n_heads, n_kv_heads, head_dim, page,
                             window, scale, softcap, sink):
-        """Prompt portions over pages of the compute type ([pages, 2, kv heads, page, head size])."""
+        """Prompt portions in float32 over pages of the compute type ([pages, 2, kv heads, page, head size])."""
         k_pool, v_pool, stride = pool[:, 0], pool[:, 1], pool.stride(0)
         rest = (n_heads, n_kv_heads, head_dim, page, window or 0, scale)
-        if self.dtype == torch.float32:
-            arguments = (_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pool), _ptr(v_pool), stride, _ptr(q_start), _ptr(kv_len),
-                         _ptr(table), table.stride(0), _ptr(item_row), 0, n_items)
-            last = (*rest, float(softcap or 0.0), _ptr(sink), 0)
-            self.launches += 1
-            if self.F32_TC_HEADS[0] <= head_dim <= self.F32_TC_HEADS[1]:
-                _check(self._tc_library().ps_prompt_attention_f32_tc(*arguments, (max_blocks + n_items) // 2, *last,
-                                                                     _ptr(self.status_flag(q.device)), _stream()), "prompt_attention_f32_tc")
-            else:
-                _check(self.core.ps_prompt_attention_f32(*arguments, max_blocks, *last, _stream()), "prompt_attention_f32")
-            return
-        pieces = dict(item_row=item_row, softcap=softcap, sink=sink)
-        if self.prefill_tc_ok(head_dim, page, q, out, pool):
-            self.prefill_attention_tc(q, out, pool.unsqueeze(1), 0, q_start, kv_len, table, 0, n_items, (max_blocks + n_items) // 2, *rest, **pieces)
+        arguments = (_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pool), _ptr(v_pool), stride, _ptr(q_start), _ptr(kv_len), _ptr(table),
+                     table.stride(0), _ptr(item_row), 0, n_items)
+        last = (*rest, float(softcap or 0.0), _ptr(sink), 0)
+        self.launches += 1
+        if self.F32_TC_HEADS[0] <= head_dim <= self.F32_TC_HEADS[1]:
+            _check(self._tc_library().ps_prompt_attention_f32_tc(*arguments, (max_blocks + n_items) // 2, *last, _ptr(self.status_flag(q.device)),
+                                                                 _stream()), "prompt_attention_f32_tc")
         else:
-            self.prefill_attention(q, out, k_pool, v_pool, stride, q_start, kv_len, table, 0, n_items, max_blocks, *rest, **pieces)
+            _check(self.core.ps_prompt_attention_f32(*arguments, max_blocks, *last, _stream()), "prompt_attention_f32")
 
     # ------------------------------------------------------------------ rotary positions + cache write
     def rotary_cache_write(self, q, k, v, inv_freq, rot_dims, interleaved, ctx, layer, n_heads, n_kv_heads,

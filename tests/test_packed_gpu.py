@@ -244,7 +244,7 @@ def test_missing_pages_are_not_seen(dtype):
 
 
 # ------------------------------------------------------------------------------------------------ portions of prompts
-PROMPT_SHAPES = [(4, 4, 64, 16), (8, 2, 128, 16), (3, 3, 64, 64), (4, 2, 64, 8), (6, 3, 96, 16), (4, 4, 48, 4), (5, 1, 80, 1), (2, 2, 128, 32)]
+PROMPT_SHAPES = [(4, 4, 64, 16), (8, 2, 128, 16), (3, 3, 64, 64), (4, 2, 64, 8), (6, 3, 96, 16), (4, 4, 48, 4), (5, 1, 80, 1), (2, 2, 128, 32), (3, 3, 20, 2)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -275,8 +275,54 @@ def test_prompt_portions(dtype, heads, kv_heads, dim, page, window, softcap, wit
             rows = slice(starts[item], starts[item + 1])
             want, weighted, sizes = attention(q[rows].double().view(-1, heads, dim), case.context(item, k), case.context(item, v),
                                               torch.arange(lengths[item] - new[item], lengths[item]), scale, window, softcap, sink)
-            limit = bound_of(want, weighted, sizes, scale, out_dtype, *((2.0 ** -9, dim, 2.0 ** -9) if dtype == BF16 else (2.0 ** -20, dim)))
+            # (bfloat16: keys, values and weights are rounded to float16, half a step of 2^-11 each)
+            limit = bound_of(want, weighted, sizes, scale, out_dtype, *((2.0 ** -10, dim, 2.0 ** -11) if dtype == BF16 else (2.0 ** -20, dim)))
             assert ((got[rows] - want).abs() <= limit).all(), (item, float(((got[rows] - want).abs() / limit).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("k_scale,v_scale,q_scale", [(1e4, 1e6, 1e-4), (1e-6, 1e-9, 1e3), (1.0, 3e30, 1.0), (1.0, 1e-30, 1.0), (3e5, 1.0, 2e5), (0.0, 0.0, 1.0),
+                                                     (1.0, 1e-3, 1e20), (1e-4, 1.0, 1e-20)])
+def test_sizes_of_numbers_in_prompts(dtype, k_scale, v_scale, q_scale):
+    """Keys, values and queries far from 1 in size: beyond float16's range on either side."""
+    ops, heads, dim, page, length, new = ops_for(dtype), 2, 64, 16, 200, 150
+    if dtype == F32 and (v_scale > 1e7 or k_scale * q_scale > 1e7):
+        pytest.skip("the kernel over float32 pages has bounds of its own")
+    case = PackedCase([length], heads, dim, page, dtype, seed=4)
+    case.k, case.v = (case.k.float() * k_scale).to(dtype), (case.v.float() * v_scale).to(dtype)
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    q = (torch.randn(new, heads * dim, generator=torch.Generator().manual_seed(2)) * q_scale).to(dtype)
+    scale = 0.125 / max(1.0, k_scale * q_scale)
+    want, weighted, sizes = attention(q.double().view(new, heads, dim), k, v, torch.arange(length - new, length), scale)
+    limit = bound_of(want, weighted, sizes, scale, dtype, *((2.0 ** -10, dim, 2.0 ** -11) if dtype == BF16 else (2.0 ** -20, dim)))
+    out = torch.empty((new, heads * dim), dtype=dtype, device=DEV)
+    ops.packed_attention_prompts(q.to(DEV), out, *planes, ints([0, new]), ints([length]), case.table.to(DEV), ints([0]), 0, 1, 3, length, heads, heads, dim,
+                                 page, None, scale)
+    assert ((out.cpu().double().view(new, heads, dim) - want).abs() <= limit).all()
+
+
+def test_nan_and_missing_pages_in_prompts():
+    """A NaN among the values reaches the rows that see it and no other; keys without a page are not seen."""
+    ops, heads, dim, page, length = ops_for(BF16), 2, 64, 16, 160
+    case = PackedCase([length, length], heads, dim, page, BF16, seed=6)
+    case.v[100, 1, 40] = float("nan")                                   # request 0, head 1, second group
+    _, planes = on_device(case)
+    table = case.table.clone()
+    table[1, 2], table[1, 5] = -1, case.pages
+    q = torch.randn(2 * length, heads * dim, generator=torch.Generator().manual_seed(3)).bfloat16()
+    out = torch.empty((2 * length, heads * dim), dtype=BF16, device=DEV)
+    ops.packed_attention_prompts(q.to(DEV), out, *planes, ints([0, length, 2 * length]), ints([length, length]), table.to(DEV), ints([0, 1]), 0, 2, 6, length,
+                                 heads, heads, dim, page, None, 0.125)
+    got = out.cpu().double().view(2, length, heads, dim)
+    bad = got[0].isnan()
+    assert bad[100:, 1, 32:].all() and bad.sum() == 60 * 32
+    k, v = (case.context(1, rows) for rows in case.held())
+    kept = torch.tensor([i for i in range(length) if i // page not in (2, 5)])
+    for i in (31, 40, 79, 90, 159):
+        mine = kept[kept <= i]
+        want, weighted, sizes = attention(q[length + i:length + i + 1].double().view(1, heads, dim), k[mine], v[mine], torch.tensor([len(mine) - 1]), 0.125)
+        assert ((got[1, i:i + 1] - want).abs() <= bound_of(want, weighted, sizes, 0.125, BF16, 2.0 ** -10, dim, 2.0 ** -11)).all()
 
 
 def test_prompts_in_several_rounds():
@@ -360,7 +406,7 @@ def test_refusals_on_the_device():
     tokens = dict(q=q, out=out, k_pool=planes[0], v_pool=planes[1], page_stride=planes[2], token_row=row, positions=at, block_table=table, n_heads=4,
                   n_kv_heads=2, head_dim=64, page_size=16, window=None, scale=0.1, max_kv_len=20)
     for change in (dict(n_heads=3), dict(q=q.float()), dict(out=out.half()), dict(out=out[:2]), dict(out=out[:, ::2]), dict(sink=torch.zeros(3, device=DEV)),
-                   dict(sink=torch.zeros(4)), dict(softcap=-1.0), dict(softcap=0.0), dict(token_row=row[:2]), dict(n_kv_heads=0)):
+                   dict(sink=torch.zeros(4)), dict(softcap=-1.0), dict(softcap=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(token_row=row[:2]), dict(n_kv_heads=0)):
         with pytest.raises(KernelError):
             ops.packed_attention_tokens(**{**tokens, **change})
     prompts = dict(q=q, out=out, k_pool=planes[0], v_pool=planes[1], page_stride=planes[2], q_start=ints([0, 3]), kv_len=ints([20]), block_table=table,
