@@ -3,12 +3,11 @@
 //
 // One CTA per (block of 256 query tokens of one request, head), tiles of 128 keys aligned to absolute positions. The block is two tiles of 128
 // queries that take turns: while the rows of one form their weights, the tensor cores work for the other.
-//   warps 0..3   a key a thread: its codes and scales come to registers a tile ahead, become low + code * step (one rounding to float16, 2^-12 of
-//                the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact as its own)
-//                and go to the swizzled tile, 16 bytes a word of codes; before that the second query tile's rows
-//   warps 4..7   the same of the values and the first query tile
-//   warps 8, 17  issue of S = Q K^T and O += P V for the first and the second query tile (8: TMEM allocation, too)
-//   warps 9..16  softmax, a thread per query row: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves, and O with it, only when
+//   warps 0..3   a key and its value a thread: codes and scales come to registers ahead of their tile, become low + code * step (one rounding to float16,
+//                2^-12 of the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact as
+//                its own) and go to the swizzled tile, 16 bytes a word of codes; before that the queries' rows
+//   warps 4, 13  issue of S = Q K^T and O += P V for the first and the second query tile (4: TMEM allocation, too)
+//   warps 5..12  softmax, a thread per query row: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves, and O with it, only when
 //                a score is beyond it by 2^8, which float16 has room for
 // A tile's keys go through in two halves of 64, whose scores have columns of their own: P of a half takes the place of its scores, P V of the half is
 // issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half. Rows hardly wait, then.
@@ -28,7 +27,7 @@ namespace packedtc {
 
 using namespace packed;
 
-constexpr int BQ = 128, BKEY = 128, MAKERS = 128, THREADS = 2 * MAKERS + 64 + 2 * BQ;                  // MAKERS: of keys, and of values
+constexpr int BQ = 128, BKEY = 128, MAKERS = 128, THREADS = MAKERS + 64 + 2 * BQ;
 constexpr uint64_t WAIT_LIMIT_NS = 200ull * 1000 * 1000;
 constexpr float MOST = 60000.f, LEAST = 0.001953125f;              // sizes of numbers that float16 holds to 2^-12 of the largest
 
@@ -308,7 +307,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         sizes_s[0] = sizes_s[1] = sizes_s[2] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)L::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -317,39 +316,34 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp < 8) {
-        // ------------------------------------------------ makers: thread r has key r of every tile, and row r of the second query tile, or the value and
-        // row of the first
-        const int r = threadIdx.x & 127;
-        const bool values = warp >= 4;
-        const unsigned char* pool = (values ? cache.v_pool : cache.k_pool) + head_at;
-        uint4 codes[GROUPS_MOST], next_codes[GROUPS_MOST];
-        uint32_t scales[GROUPS_MOST], next_scales[GROUPS_MOST];
+    if (warp < 4) {
+        // ------------------------------------------------ makers: thread r has key r of every tile and its value, and row r of both query tiles
+        const int r = threadIdx.x;
+        uint4 k_codes[GROUPS_MOST], v_codes[GROUPS_MOST];
+        uint32_t k_scales[GROUPS_MOST], v_scales[GROUPS_MOST];
         bool strange = false;
-        float most_size = 0.f;
-        auto fetch = [&](int kb) {
+        float k_most = 0.f, v_most = 0.f;
+        long long page_at = -1;                                    // of the key whose numbers are asked for (below 0: not needed, or no page)
+        int page_row = 0;
+        auto locate = [&](int kb) {
             const int key = kb * BKEY + r;
             const bool needed = key >= lo && key <= hi;
             const int page = needed ? cache.pages.of(table_row, key) : -1;
             strange |= needed && page < 0;
-            const int row = key & (page_size - 1);
-            const unsigned char* at = pool + (long long)page * cache.page_stride;
-#pragma unroll
-            for (int j = 0; j < GROUPS_MOST; ++j) {
-                const bool there = page >= 0 && j < groups;
-                next_codes[j] = there ? *reinterpret_cast<const uint4*>(at + (row * groups + j) * 16) : make_uint4(0, 0, 0, 0);
-                next_scales[j] = there ? *reinterpret_cast<const uint32_t*>(at + page_size * groups * 16 + (row * groups + j) * 4) : 0u;
-            }
+            page_row = key & (page_size - 1);
+            page_at = page < 0 ? -1 : (long long)page * cache.page_stride + head_at;
         };
-        auto take = [&]() {
+        auto fetch = [&](const unsigned char* pool, uint4 (&codes)[GROUPS_MOST], uint32_t (&scales)[GROUPS_MOST]) {
+            const unsigned char* at = pool + page_at;
 #pragma unroll
             for (int j = 0; j < GROUPS_MOST; ++j) {
-                codes[j] = next_codes[j];
-                scales[j] = next_scales[j];
+                const bool there = page_at >= 0 && j < groups;
+                codes[j] = there ? *reinterpret_cast<const uint4*>(at + (page_row * groups + j) * 16) : make_uint4(0, 0, 0, 0);
+                scales[j] = there ? *reinterpret_cast<const uint32_t*>(at + page_size * groups * 16 + (page_row * groups + j) * 4) : 0u;
             }
         };
         // a row of a tile: place p of the codes (part p / groups of group p % groups) becomes eight numbers; what is not there becomes zeros
-        auto make = [&](unsigned char* tile) {
+        auto make = [&](unsigned char* tile, const uint4 (&codes)[GROUPS_MOST], const uint32_t (&scales)[GROUPS_MOST], float& most_size) {
             uint32_t step[GROUPS_MOST], low[GROUPS_MOST];
 #pragma unroll
             for (int j = 0; j < GROUPS_MOST; ++j) {
@@ -379,78 +373,95 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        fetch(kb_first);
-        {
-            const int x = values ? 0 : 1, place = x * BQ + r;
+        // (in front of the queries' rows where registers do for both)
+        locate(kb_first);
+        if constexpr (HD == 64) {
+            fetch(cache.k_pool, k_codes, k_scales);
+            fetch(cache.v_pool, v_codes, v_scales);
+        }
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+            const int place = x * BQ + r;
             const __nv_bfloat16* row = q + (long long)(tok0 + place) * q_stride + (long long)h * head_dim;
             float most = 0.f;
             bool odd = false;
-            // twice over the row: for its largest number, and for its numbers (its 128 or 256 bytes stay in L1)
-            auto load = [&](int d, float (&n)[8]) {
-                if (place < rows && aligned_q && d < head_dim) {
-                    const uint4 raw = *reinterpret_cast<const uint4*>(row + d);
-                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint4 raw[HD / 8];                                     // the whole row at once: its loads are under way together
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        n[2 * i] = __uint_as_float(w[i] << 16);
-                        n[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            for (int i = 0; i < HD / 8; ++i) {
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (place < rows && 8 * i < head_dim) {
+                    if (aligned_q) {
+                        raw[i] = *reinterpret_cast<const uint4*>(row + 8 * i);
+                    } else {
+                        const unsigned short* at = reinterpret_cast<const unsigned short*>(row + 8 * i);
+                        auto number = [&](int j) -> uint32_t { return 8 * i + j < head_dim ? at[j] : 0u; };
+                        raw[i] = make_uint4(number(0) | number(1) << 16, number(2) | number(3) << 16, number(4) | number(5) << 16, number(6) | number(7) << 16);
                     }
-                } else {
+                }
+            }
+            auto each = [&](auto f) {                              // two neighbouring numbers to a word
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) n[i] = place < rows && d + i < head_dim ? __bfloat162float(row[d + i]) : 0.f;
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = f(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+                    raw[i] = make_uint4(v[0], v[1], v[2], v[3]);
                 }
             };
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float n[8];
-                load(d, n);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    most = fmaxf(most, fabsf(n[i]));
-                    odd |= !(fabsf(n[i]) <= 3.4028235e38f);
+            for (int i = 0; i < HD / 8; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float lo_half = fabsf(__uint_as_float(w[j] << 16)), hi_half = fabsf(__uint_as_float(w[j] & 0xffff0000u));
+                    most = max3(most, lo_half, hi_half);
+                    odd |= !(lo_half <= 3.4028235e38f) || !(hi_half <= 3.4028235e38f);
                 }
             }
             // 2^up brings the largest to [256, 512); a NaN or infinity stays one
             const int up = most > 0.f && !odd ? min(126, 135 - max(1, (int)(__float_as_uint(most) >> 23))) : 0;
             const float by = __uint_as_float((uint32_t)(127 + up) << 23);
             factor_s[place] = __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float n[8];
-                load(d, n);
-                uint4 v;
-                v.x = half_pair(n[0] * by, n[1] * by);
-                v.y = half_pair(n[2] * by, n[3] * by);
-                v.z = half_pair(n[4] * by, n[5] * by);
-                v.w = half_pair(n[6] * by, n[7] * by);
-                *reinterpret_cast<uint4*>(q_s + x * L::Q_BYTES + tile_byte(r, d)) = v;
-            }
+            each([&](float a, float b) { return half_pair(a * by, b * by); });
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<uint4*>(q_s + x * L::Q_BYTES + tile_byte(r, 8 * i)) = raw[i];
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&q_full[x]);
         }
-        uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+        if constexpr (HD != 64) {
+            fetch(cache.k_pool, k_codes, k_scales);
+            fetch(cache.v_pool, v_codes, v_scales);
+        }
         uint32_t it = 0;
         for (int kb = kb_first; kb <= kb_last; ++kb, ++it) {
             const int s = it % KV_STAGES;
-            take();
-            if (kb < kb_last) fetch(kb + 1);
-            if (!mbar_wait(&empty[s], ((it / KV_STAGES) & 1) ^ 1, abort_flag)) { if (lane == 0) atomicExch(status, values ? 52 : 51); break; }
-            make(kv_s + (size_t)s * L::STAGE_BYTES + (values ? L::KV_BYTES : 0));
-            mbar_arrive(&full[s]);
+            const uint32_t free = ((it / KV_STAGES) & 1) ^ 1;
+            unsigned char* tile = kv_s + (size_t)s * L::STAGE_BYTES;
+            if (kb < kb_last) locate(kb + 1);
+            if (!mbar_wait(&k_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 51); break; }
+            make(tile, k_codes, k_scales, k_most);
+            mbar_arrive(&k_full[s]);
+            if (kb < kb_last) fetch(cache.k_pool, k_codes, k_scales);
+            if (!mbar_wait(&v_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 52); break; }
+            make(tile + L::KV_BYTES, v_codes, v_scales, v_most);
+            mbar_arrive(&v_full[s]);
+            if (kb < kb_last) fetch(cache.v_pool, v_codes, v_scales);
         }
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most_size));
+        const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_most)), v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_most));
         const bool any = __any_sync(0xffffffffu, strange);
         if (lane == 0) {
-            atomicMax(&sizes_s[values ? 1 : 0], bits);
+            atomicMax(&sizes_s[0], k_bits);
+            atomicMax(&sizes_s[1], v_bits);
             if (any) atomicExch(&sizes_s[2], 1u);
         }
-    } else if (warp == 8 || warp == 17) {
+    } else if (warp == 4 || warp == 13) {
         // ------------------------------------------------ MMA issuers, one for each query tile
         // D f32, A/B f16: S = Q K^T both K-major, N = 64; O = P V with A from TMEM and B MN-major (bit 16), N = HD
         constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
         constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
         const uint32_t one = lane == 0 ? 1u : 0u;
-        const int x = warp == 8 ? 0 : 1, first = first_of(x), last = last_of(x);
+        const int x = warp == 4 ? 0 : 1, first = first_of(x), last = last_of(x);
         const uint32_t s_at = tmem_base + L::S_COL + x * 128, o_at = tmem_base + L::O_COL + x * HD;
         const uint64_t q_desc = desc_sw128(smem_u32(q_s + x * L::Q_BYTES), 16);
         auto waits = [&](uint64_t* bar, uint32_t parity, int code) {
@@ -497,7 +508,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         }
     } else {
         // ------------------------------------------------ rows
-        const int quarter = warp & 3, x = (warp - 9) >> 2;
+        const int quarter = warp & 3, x = (warp - 5) >> 2;
         const int r = quarter * 32 + lane, place = x * BQ + r, pos = pos0 + place;
         const int first = first_of(x), last = last_of(x);
         const int lo_row = pos < 0 ? 0 : first_visible_key(pos, window);
@@ -630,7 +641,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 4) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)L::TMEM_COLS) : "memory");
     }
