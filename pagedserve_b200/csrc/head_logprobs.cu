@@ -22,6 +22,8 @@ namespace headlp {
 
 using namespace logprob;
 
+constexpr int NT = 256, CHUNK = NT * PER, CAPACITY = capacity<NT>();
+
 constexpr int BM = 128, BN = 256, BK = 64, TEAMS = 4, ROW_THREADS = 128 * TEAMS, HEAD_THREADS = 64 + ROW_THREADS;
 constexpr int STAGE_BYTES = BM * BK * 2 + (BN / 2) * BK * 2;
 constexpr int HELD = 16;                                           // entries that a row's thread holds before it sends them to the row's list
@@ -155,10 +157,10 @@ sample_kernel(const float* __restrict__ logits, long long ld, int n, int every, 
             x[u] = i < n ? logits[r * ld + i] : -INFINITY;
             big = fmaxf(big, x[u]);
         }
-        consider(list, x, chunk, n, big, top);
+        consider<NT>(list, x, big, top, [&](int u) { const int i = chunk + u * NT + tid; return i < n ? i : -1; });
     }
     __syncthreads();
-    rank(list, top);
+    rank<NT>(list, top);
     if (tid < top) {
         const unsigned long long entry = entry_s[tid];
         out.list[r * LIST + tid] = entry_of(order_in(entry), index_in(entry) * every);
@@ -422,7 +424,7 @@ join_kernel(const int* __restrict__ targets, int V, int strips, int top, int eve
                 else entry_s[i] = (int)(uint32_t)entry % every == 0 ? 0ull : entry_of(order_of(__uint_as_float((uint32_t)(entry >> 32))), (int)(uint32_t)entry);
             }
             __syncthreads();
-            rank(list, top);
+            rank<NT>(list, top);
         } else {
             __syncthreads();
             for (int chunk = 0; chunk < V; chunk += CHUNK) {
@@ -442,10 +444,10 @@ join_kernel(const int* __restrict__ targets, int V, int strips, int top, int eve
                     v[u] = chunk + i < end ? logit_s[i] : -INFINITY;
                     big = fmaxf(big, v[u]);
                 }
-                consider(list, v, chunk, end, big, top);
+                consider<NT>(list, v, big, top, [&](int u) { const int i = chunk + u * NT + tid; return i < end ? i : -1; });
                 __syncthreads();
             }
-            rank(list, top);
+            rank<NT>(list, top);
         }
     }
     // the strips' sums, by the first warp

@@ -6,10 +6,10 @@
 namespace ps {
 namespace logprob {
 
-constexpr int NT = 256, PER = 8, CHUNK = NT * PER, MOST_TOP = 32, RANK_AT = 128, GROUPS = NT / 4;
+constexpr int PER = 8, MOST_TOP = 32, RANK_AT = 128, GROUPS = 64;      // (a chunk: PER numbers of every thread of a CTA, NT of them)
 constexpr int DIRECT = 32;                                       // threads of a chunk that may add what they have without a new bound
 constexpr int THIN_FROM = 96;                                    // entries of a list from which the bound is applied to it, too
-constexpr int CAPACITY = MOST_TOP + RANK_AT + CHUNK;
+template <int NT> constexpr int capacity() { return MOST_TOP + RANK_AT + NT * PER; }
 constexpr float LEAST = -1000.f;                                  // e^LEAST is 0, and LEAST times that too
 
 // whole numbers in the order of the floats; 1: a NaN, behind everything; 0: nothing there
@@ -58,7 +58,7 @@ struct Results {
 
 // The list of a CTA: entries [0, count), of which the first `top` are ranked after rank().
 struct List {
-    unsigned long long* entry;  // [CAPACITY]
+    unsigned long long* entry;  // [capacity]
     unsigned long long* kept;   // [MOST_TOP]
     int* count;
     uint32_t* limit;            // an entry joins if its order is beyond this one (0: the list has fewer than `top`)
@@ -67,11 +67,13 @@ struct List {
 };
 // Sets *list.bound to a number's order that at least `top` of the numbers in hand reach, or to 0; `most`: the largest order of this thread's (0:
 // it has none).  All threads; ends with the bound visible.
+template <int NT>
 __device__ __forceinline__ void find_bound(const List& list, uint32_t most, int top) {
+    constexpr int LANES = NT / GROUPS;                            // threads of a group
     const int tid = threadIdx.x;
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    if ((tid & 3) == 0) list.group[tid >> 2] = most;
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (tid % LANES == 0) list.group[tid / LANES] = most;
     __syncthreads();
     if (tid < GROUPS) {
         const uint32_t own = list.group[tid];
@@ -82,10 +84,11 @@ __device__ __forceinline__ void find_bound(const List& list, uint32_t most, int 
     __syncthreads();
 }
 // all threads; begins and ends with the list complete and visible
+template <int NT>
 __device__ __forceinline__ void rank(const List& list, int top) {
     int n = *list.count;
     if (n > THIN_FROM) {                                          // a long list: what is below the bound goes first
-        constexpr int EACH = (CAPACITY + NT - 1) / NT;
+        constexpr int EACH = (capacity<NT>() + NT - 1) / NT;
         unsigned long long mine[EACH];
         uint32_t most = 0;
 #pragma unroll
@@ -94,7 +97,7 @@ __device__ __forceinline__ void rank(const List& list, int top) {
             mine[i] = at < n ? list.entry[at] : 0ull;
             most = max(most, order_in(mine[i]));
         }
-        find_bound(list, most, top);                              // (everyone has read its entries)
+        find_bound<NT>(list, most, top);                          // (everyone has read its entries)
         if (threadIdx.x == 0) *list.count = 0;
         __syncthreads();
         const uint32_t from = max(*list.bound, 1u);
@@ -119,10 +122,10 @@ __device__ __forceinline__ void rank(const List& list, int top) {
     __syncthreads();
 }
 
-// The numbers of a chunk, PER of each thread (the u-th of thread t is chunk + u * NT + t; `end`: one past the last that is there; `big`: the
-// thread's largest), to the list if they belong there.  All threads.
-__device__ __forceinline__ void consider(const List& list, const float (&x)[PER], int chunk, int end, float big, int top) {
-    const int tid = threadIdx.x;
+// The numbers of a chunk, PER of each thread, to the list if they belong there; at(u): the index of the u-th of them, below 0 where there is none; `big`: the
+// largest.  All threads.
+template <int NT, typename At>
+__device__ __forceinline__ void consider(const List& list, const float (&x)[PER], float big, int top, At at) {
     const uint32_t limit = *list.limit;
     const bool hit = limit <= 1u || order_of(big) > limit;        // (an open list takes everything)
     const int hits = __syncthreads_count(hit);
@@ -132,22 +135,20 @@ __device__ __forceinline__ void consider(const List& list, const float (&x)[PER]
         uint32_t most = 0;
 #pragma unroll
         for (int u = 0; u < PER; ++u)
-            if (chunk + u * NT + tid < end) most = max(most, order_of(x[u]));
-        find_bound(list, most, top);
+            if (at(u) >= 0) most = max(most, order_of(x[u]));
+        find_bound<NT>(list, most, top);
         from = max(from, max(*list.bound, 1u));
     }
     if (hit || hits > DIRECT) {
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int i = chunk + u * NT + tid;
-            if (i < end) {
+        for (int u = 0; u < PER; ++u)
+            if (at(u) >= 0) {
                 const uint32_t order = order_of(x[u]);
-                if (order >= from) list.entry[atomicAdd(list.count, 1)] = entry_of(order, i);
+                if (order >= from) list.entry[atomicAdd(list.count, 1)] = entry_of(order, at(u));
             }
-        }
     }
     __syncthreads();
-    if (hits > DIRECT || *list.count > top + RANK_AT) rank(list, top);
+    if (hits > DIRECT || *list.count > top + RANK_AT) rank<NT>(list, top);
 }
 
 }  // namespace logprob

@@ -2294,8 +2294,8 @@ class Ops:
         if not (0 <= top <= min(vocabulary, MOST_ALTERNATIVES)):
             raise KernelError(f"{what}: top is 0 to {MOST_ALTERNATIVES}, and at most the vocabulary")
         self._on_current_device(what, targets)
-        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)
-        return TokenLogprobs(new((rows,), torch.float32), new((rows,), torch.float32), new((rows, top), torch.float32), new((rows, top), torch.int32))
+        numbers = torch.empty((2 + top, rows), dtype=torch.float32, device=device)
+        return TokenLogprobs(numbers[0], numbers[1], numbers[2:].view(rows, top), targets.new_empty((rows, top)))
 
     def token_logprobs(self, logits, targets, top=0, status=None, results=None):
         """:class:`TokenLogprobs` of float32 ``logits`` [rows, vocabulary] and one token a row (int32): its log probability under the row's softmax,
