@@ -45,62 +45,102 @@ template <> struct Eight<float> {
     }
 };
 
-// thread = (token, k or v, head, group, part of the group); `aligned`: every part is whole 16-byte pieces of its row
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The codes of eight numbers as a word. Quotients by the reciprocal are within 2e-6 of the rounded ones: they name the same code unless one of them is
+// near half a code, where the divisions decide. (The codes are 0 to 15 by themselves: low is not above a number, 15 steps from it not below.) Four codes add up to 16
+// bits in float32, exactly.
+__device__ __forceinline__ uint32_t word_of(const float (&x)[8], float low, float step) {
+    if (!(step > 0.f)) return 0u;
+    const float reciprocal = __frcp_rn(step);
+    float code[8], off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float quotient = __fsub_rn(x[i], low) * reciprocal;
+        code[i] = __fadd_rn(__fadd_rn(quotient, 12582912.f), -12582912.f);        // (1.5 * 2^23: the nearest whole number, ties to even)
+        off = fmaxf(off, fabsf(quotient - code[i]));
+    }
+    if (!(off <= 0.4999f) || step < 1e-30f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], low), step)), 0.f), 15.f);
+    const float even = fmaf(fmaf(fmaf(code[6], 16.f, code[4]), 16.f, code[2]), 16.f, code[0]);
+    const float odd = fmaf(fmaf(fmaf(code[7], 16.f, code[5]), 16.f, code[3]), 16.f, code[1]);
+    return __byte_perm(__float_as_uint(even + 8388608.f), __float_as_uint(odd + 8388608.f), 0x5410);
+}
+
+// A token's parts (k or v, head, group, part of the group) over the threads of blockIdx.y = 0, 1, ..; `aligned`: every part is whole 16-byte pieces of its
+// row.  What bounds it is instructions, about 150 a thread (3,400 rows of 25 heads of 64 in float32: 30 us with an index over the parts of all tokens, a division and
+// a shift for every number, 26 without that index, so 20; several tokens a thread gained nothing).
 template <typename T>
 __global__ void __launch_bounds__(256)
 append_kernel(const T* __restrict__ k_src, long long k_stride, const T* __restrict__ v_src, long long v_stride,
               const int* __restrict__ token_row, const int* __restrict__ positions, Pages pages, unsigned char* __restrict__ k_pool,
-              unsigned char* __restrict__ v_pool, long long page_stride, int tokens, int planes, int n_kv_heads, int head_dim, int aligned) {
+              unsigned char* __restrict__ v_pool, long long page_stride, int planes, int n_kv_heads, int head_dim, int aligned) {
     pdl_prologue();
     k_src = pdl_fresh(k_src);
     v_src = pdl_fresh(v_src);
-    const int groups = groups_of(head_dim), per_plane = n_kv_heads * groups * 4;
-    const long long index = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool there = index < (long long)tokens * planes * per_plane;          // (the lanes of a group are there together)
-    const long long row_index = there ? index / per_plane : 0;
-    const int inside = there ? (int)(index - row_index * per_plane) : 0;
-    const int t = (int)(row_index / planes), plane = planes == 2 ? (int)(row_index & 1) : (k_src ? 0 : 1);
-    const int part = inside & 3, j = (inside >> 2) % groups, head = (inside >> 2) / groups;
+    const int groups = groups_of(head_dim), per_plane = n_kv_heads * groups * 4, t = blockIdx.x;
+    const int index = blockIdx.y * blockDim.x + threadIdx.x;
+    const bool there = index < planes * per_plane;                               // (the lanes of a group are there together)
+    const int second = planes == 2 && index >= per_plane ? 1 : 0, inside = there ? index - second * per_plane : 0;
+    const int plane = planes == 2 ? second : (k_src ? 0 : 1);
+    const int p = positions[t], table_row = token_row[t];
+    const int part = inside & 3, head = (inside >> 2) / groups, j = (inside >> 2) - head * groups;
     const int d = j * GROUP + part * 8;
     const int count = there ? min(8, head_dim - d) : 0;                          // numbers of this part that exist (may be negative)
-    const T* src = (plane ? v_src + t * v_stride : k_src + t * k_stride) + head * head_dim + d;
-    float x[8];
+    const T* src = (plane ? v_src + t * v_stride : k_src + t * k_stride) + (head * head_dim + d);
+    float x[8], low = INFINITY, high = -INFINITY;
+    bool bad = false;                                                            // (minimum and maximum pass NaN over)
+    if (count == 8) {
+        if (aligned) {
+            Eight<T>::load(src, x);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (count == 8 && aligned) {
-        Eight<T>::load(src, x);
+            for (int i = 0; i < 8; ++i) x[i] = to_float(src[i]);
+        }
+        low = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
+        high = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
+        float zero = 0.f;                                                        // 0, or NaN where a number is one or an infinity
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zero = fmaf(x[i], 0.f, zero);
+        bad = zero != 0.f;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) x[i] = to_float(src[i]);
-    }
-    float low = INFINITY, high = -INFINITY;
-    bool bad = false;                                                            // (fminf and fmaxf pass NaN over)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < count) {
-            low = fminf(low, x[i]);
-            high = fmaxf(high, x[i]);
-            bad |= x[i] != x[i];
+        for (int i = 0; i < 8; ++i) {
+            x[i] = 0.f;
+            if (i < count) {
+                x[i] = to_float(src[i]);
+                low = fminf(low, x[i]);
+                high = fmaxf(high, x[i]);
+                bad |= x[i] != x[i];
+            }
         }
+    }
     if (bad) low = -INFINITY;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
-    if (!there) return;
-    const int p = positions[t], page = pages.of(token_row[t], p);
-    if (page < 0) return;
+    const int page = pages.of(table_row, p);                                     // (looked up while the numbers are on their way)
+    if (!there || page < 0) return;
     low = bf16_below(low);
     float step = bf16_above(__fdiv_rn(__fsub_rn(high, low), 15.0f));
     uint32_t word = 0;
     if (isfinite(low) && isfinite(step)) {
+        if (count < 8)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float code = step > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], low), step)), 0.f), 15.f) : 0.f;
-            if (i < count) word |= (uint32_t)(int)code << code_shift(i);
-        }
+            for (int i = 0; i < 8; ++i)
+                if (i >= count) x[i] = low;                                       // (code 0)
+        word = word_of(x, low, step);
     } else {
         low = step = __uint_as_float(0x7fff0000u);
     }
@@ -112,8 +152,9 @@ append_kernel(const T* __restrict__ k_src, long long k_stride, const T* __restri
             (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
 }
 
-// thread = (item, position, k or v, head, word); out: pages [n_items * span / out_page, 2, kv heads, out_page, head_dim], item i's
-// position p in page i * span / out_page + p / out_page. Positions from kv_len on are left as they are.
+// A position's words (k or v, head, place in the row) over the threads of a CTA, blockIdx.x = position, blockIdx.y = item; out: pages
+// [n_items * span / out_page, 2, kv heads, out_page, head_dim], item i's position p in page i * span / out_page + p / out_page. Positions from kv_len on
+// are left as they are.
 template <typename T>
 __global__ void __launch_bounds__(256)
 unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
@@ -123,35 +164,31 @@ unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __r
     k_pool = pdl_fresh(k_pool);
     v_pool = pdl_fresh(v_pool);
     const int groups = groups_of(head_dim), words = groups * 4, per_row = 2 * n_kv_heads * words;
-    const int item = blockIdx.y;
-    const long long index = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long position64 = index / per_row;
-    if (position64 >= span) return;
-    const int p = (int)position64;
+    const int item = blockIdx.y, p = blockIdx.x;
     if (p >= kv_len[item]) return;
     const int page = pages.of(item_row ? item_row[item] : item, p);
     if (page < 0) return;
-    int rest = (int)(index - position64 * per_row);
-    const int place = rest % words, plane = rest / words % 2, head = rest / words / 2;
-    const int j = place % groups, d = j * GROUP + place / groups * 8;
-    const int page_size = 1 << pages.page_log2, row = p & (page_size - 1);
-    const unsigned char* slab = (plane ? v_pool : k_pool) + (long long)page * page_stride + (long long)head * slab_bytes(page_size, head_dim);
-    const uint32_t word = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
-    const uint32_t scale = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
-    const float step = step_of(scale), low = low_of(scale);
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word >> code_shift(i)) & 15u), step, low);
-    const int out_size = 1 << out_log2;
+    const int page_size = 1 << pages.page_log2, row = p & (page_size - 1), out_size = 1 << out_log2;
     const long long out_page = (long long)item * (span >> out_log2) + (p >> out_log2);
-    T* to = out + (((out_page * 2 + plane) * n_kv_heads + head) * out_size + (p & (out_size - 1))) * head_dim + d;
-    const int count = head_dim - d;
-    if (count >= 8 && aligned) {
-        Eight<T>::store(to, x);
-    } else {
+    for (int index = threadIdx.x; index < per_row; index += blockDim.x) {
+        const int both = index / words, place = index - both * words, plane = both >= n_kv_heads ? 1 : 0, head = both - plane * n_kv_heads;
+        const int part = place / groups, j = place - part * groups, d = j * GROUP + part * 8;
+        const unsigned char* slab = (plane ? v_pool : k_pool) + (long long)page * page_stride + (long long)head * slab_bytes(page_size, head_dim);
+        const uint32_t word = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
+        const uint32_t scale = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
+        const float step = step_of(scale), low = low_of(scale);
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) to[i] = from_float<T>(x[i]);
+        for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word >> code_shift(i)) & 15u), step, low);
+        T* to = out + (((out_page * 2 + plane) * n_kv_heads + head) * out_size + (p & (out_size - 1))) * head_dim + d;
+        const int count = head_dim - d;
+        if (count >= 8 && aligned) {
+            Eight<T>::store(to, x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < count) to[i] = from_float<T>(x[i]);
+        }
     }
 }
 
@@ -159,22 +196,24 @@ template <typename T>
 int append(const void* k_src, long long k_stride, const void* v_src, long long v_stride, const int* token_row, const int* positions,
            const Pages& pages, void* k_pool, void* v_pool, long long page_stride, int tokens, int n_kv_heads, int head_dim, cudaStream_t s) {
     const int planes = (k_src ? 1 : 0) + (v_src ? 1 : 0);
-    const long long threads = (long long)tokens * planes * n_kv_heads * groups_of(head_dim) * 4;
-    if ((threads + 255) / 256 > 0x7fffffffll) return PS_ERR_UNSUPPORTED;
+    const long long parts = (long long)planes * n_kv_heads * groups_of(head_dim) * 4;
+    const int threads = parts >= 256 ? 256 : (int)((parts + 31) / 32 * 32);
+    if ((parts + threads - 1) / threads > 65535) return PS_ERR_UNSUPPORTED;
     constexpr int PER = 16 / (int)sizeof(T);
     const int aligned = !(((uintptr_t)k_src | (uintptr_t)v_src) & 15) && k_stride % PER == 0 && v_stride % PER == 0 && head_dim % 8 == 0;
-    return launch_pdl(append_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, (const T*)k_src, k_stride, (const T*)v_src,
-                      v_stride, token_row, positions, pages, (unsigned char*)k_pool, (unsigned char*)v_pool, page_stride, tokens, planes,
+    return launch_pdl(append_kernel<T>, dim3(tokens, (unsigned)((parts + threads - 1) / threads)), dim3(threads), 0, s, (const T*)k_src, k_stride,
+                      (const T*)v_src, v_stride, token_row, positions, pages, (unsigned char*)k_pool, (unsigned char*)v_pool, page_stride, planes,
                       n_kv_heads, head_dim, aligned);
 }
 
 template <typename T>
 int unpack(const void* k_pool, const void* v_pool, long long page_stride, const int* kv_len, const int* item_row, const Pages& pages, int n_items,
            int span, void* out, int out_page, int n_kv_heads, int head_dim, cudaStream_t s) {
-    const long long threads = (long long)span * 2 * n_kv_heads * groups_of(head_dim) * 4;
-    if ((threads + 255) / 256 > 0x7fffffffll) return PS_ERR_UNSUPPORTED;
+    const long long words = (long long)2 * n_kv_heads * groups_of(head_dim) * 4;
+    const int threads = words >= 256 ? 256 : (int)((words + 31) / 32 * 32);
+    if (words > 0x7fffffff) return PS_ERR_UNSUPPORTED;
     const int aligned = !((uintptr_t)out & 15) && head_dim % 8 == 0;
-    return launch_pdl(unpack_kernel<T>, dim3((unsigned)((threads + 255) / 256), n_items), dim3(256), 0, s, (const unsigned char*)k_pool,
+    return launch_pdl(unpack_kernel<T>, dim3(span, n_items), dim3(threads), 0, s, (const unsigned char*)k_pool,
                       (const unsigned char*)v_pool, page_stride, kv_len, item_row, pages, span, (T*)out, log2_of(out_page), n_kv_heads, head_dim,
                       aligned);
 }

@@ -47,6 +47,23 @@ def test_written_bytes(dtype, kv_heads, dim, page):
     assert torch.equal(got.cpu()[..., :page * groups * 20], want[..., :page * groups * 20])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kv_heads,dim,page", [(25, 64, 16), (3, 33, 4), (8, 128, 64)])
+def test_written_bytes_of_many_tokens(dtype, kv_heads, dim, page):
+    """Tokens enough that a CTA takes several, a number of them that is no multiple of four, some without a place."""
+    ops, case = ops_for(dtype), PackedCase([1501, 700, 3], kv_heads, dim, page, dtype, seed=dim)
+    got = case.pool.to(DEV)
+    positions = case.positions.clone()
+    positions[5::7] = -1
+    ops.kv_append_packed(case.k.flatten(1).to(DEV), case.v.flatten(1).to(DEV), case.token_row.to(DEV), positions.to(DEV), case.table.to(DEV), got[:, 0],
+                         got[:, 1], got.stride(0), kv_heads, dim, page)
+    keep = torch.ones(len(positions), dtype=torch.bool)
+    keep[5::7] = False
+    case.k, case.v, case.token_row, case.positions = case.k[keep], case.v[keep], case.token_row[keep], case.positions[keep]
+    groups = -(-dim // 32)
+    assert torch.equal(got.cpu()[..., :page * groups * 20], case.filled()[..., :page * groups * 20])
+
+
 def special_rows(dim):
     g = torch.Generator().manual_seed(5)
     rows = [torch.zeros(dim), torch.full((dim,), 3.25), torch.full((dim,), -1.0000001), torch.randn(dim, generator=g) * 1e-30,
