@@ -17,8 +17,11 @@
 // A CTA has a token, a key head (8 or 16 of its query heads) and a share of the keys; a warp takes tiles of 16 keys, which it brings to shared
 // memory itself (cp.async, a ring of its own, no barrier). Shares are a cluster and merge through shared memory.
 //
-// What bounds it: instructions. A tile of 16 keys of 64 numbers (1,280 bytes) takes about 170 a warp, 52 of them the masks and shifts, which run
-// at half rate; 8 and 4 mma.sync are 84 clocks of a tensor core that is otherwise idle.
+// What bounds it: instructions, not bytes (the same time with one page that every token shares). A tile of 16 keys is about 600 instructions a warp at
+// 128 numbers a head and 8 queries, half of them masks, shifts and sums on the ALU pipe, which issues every other clock (44 - 51 % busy; a warp's own chain
+// of scores, weights and products leaves the rest idle); its 32 mma.sync are not felt. 64 tokens of 4,099 keys, 32 heads on 8 of 128: 102 us, 2.3 TB/s;
+// 64 x 1,024, 12 heads of 64: 28 us; one token of 32,768: 36 us, 12 CTAs a cluster share of 8 on 148 SMs. A page's number is asked for a tile before it
+// is used and not compared until then, or its latency stands in the loop (110 and 46 us).
 #include "packed.cuh"
 
 namespace ps {
@@ -123,10 +126,12 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     const int step_tiles = shares * M_WARPS;
     int tile = lo / M_KEYS + share * M_WARPS + warp, ahead = tile;
     uint32_t paged = 0;                                                          // (by_tile) the stages whose tile has a page
-    auto page_of = [&](int which) { return by_tile && which * M_KEYS <= last ? pages.of(table_row, which * M_KEYS) : -1; };
-    int next_page = page_of(ahead);                                              // asked for a tile before it is needed
+    // (a tile's page is asked for a tile before, and not looked at until then: a comparison here would wait for it)
+    const int* table = pages.block_table + (size_t)table_row * pages.bt_stride;
+    auto page_of = [&](int which) { return by_tile && which * M_KEYS <= last ? table[which * M_KEYS >> pages.page_log2] : -1; };
+    int next_page = page_of(ahead);
     auto fetch = [&](int which, int stage) {
-        const int key0 = which * M_KEYS, page = next_page;
+        const int key0 = which * M_KEYS, page = next_page < pages.n_pages ? next_page : -1;
         next_page = page_of(which + step_tiles);
         paged &= ~(1u << stage);
         if (key0 <= last) {

@@ -1312,9 +1312,12 @@ class Ops:
         self.launches += 1
         if self.dtype == torch.bfloat16 and head_dim <= 128:
             if not shares:
-                ctas, most = T * n_kv_heads * -(-n_heads // n_kv_heads // 16), keys // 128
-                shares = 1
-                while shares < 8 and ctas * shares * 2 <= 1184 and shares * 2 <= most:
+                # Shares pay while the GPU has SMs without a CTA, from 128 keys each on, and beyond that (to 8 CTAs an SM) only where a share is
+                # long against their merge. Measured in us at 1, 2, 4, 8 shares: 8 x 1,024 keys (12 heads of 64) 11.5, 9.3, 9.6, 13.1;
+                # 1 x 32,768 244, 126, 66, 36; 64 x 1,024 28.2, 31.0, 43.7, 73.2; 64 x 4,099 (32 heads on 8 of 128) 120, 102, 107, 130.
+                ctas, shares = T * n_kv_heads * -(-n_heads // n_kv_heads // 16), 1
+                while shares < 8 and (ctas * shares * 2 <= 592 and shares * 2 <= keys // 128
+                                      or ctas * shares * 2 <= 1184 and shares * 2 <= keys // 1024):
                     shares *= 2
             _check(self._packed_library().ps_packed_tokens_mma(
                 _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
