@@ -7,12 +7,13 @@
 //             the tensor pipe; a warp reads 32 tokens of its rows in about 2,300, most of them waits for results, so that with two threads a
 //             row the reading was as long as the product.
 // sample      for the most likely tokens, the logits of every s-th token (about 2,048 of them) are formed first, by the ordinary product: the `top`-th
-//             largest of them is a bound that the row's `top` largest reach.  The product sends what lies beyond it (about 25 * top of 50,257) to a
-//             list of its row: a number larger than the bound, or equal to it in front of the sampled token that set it.  A thread holds up to
-//             16 of them in shared memory before it takes places in the list, all rows of a warp together (an atomic addition for each number cost a
-//             microsecond's wait: 326 us of 445; one for each row that had eight, 157 of 266 us with 20 alternatives).
+//             largest of them is a bound that the row's `top` largest reach, less 2^-16 of itself, since another product may add in another order.
+//             The product sends what lies beyond it (about 25 * top of 50,257) to a list of its row: a number larger than the bound, or equal to it
+//             up to the sampled token that set it, so that whatever is not in the list comes behind all that is.  A thread holds up to 16 of them in
+//             shared memory before it takes places in the list, all rows of a warp together (an atomic addition for each number cost a microsecond's
+//             wait: 326 us of 445; one for each row that had eight, 157 of 266 us with 20 alternatives).
 // join        a CTA a row adds the strips' sums up, ranks the list, and writes the results.  A row whose list did not hold all (an order of tokens that
-//             fools the sample) has its logits formed again there, token by token.
+//             fools the sample), or fewer than `top`, has its logits formed again there, token by token.
 #include <cuda.h>
 
 #include "logprobs.cuh"
@@ -130,10 +131,10 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 struct Scratch {
     float* sums;                     // [rows, TEAMS * strips, 3]: m, S, W
     float* given;                    // [rows]
-    unsigned long long* list;        // [rows, LIST]: the sample's `top` as entries, then (logit, token) of others
+    unsigned long long* list;        // [rows, LIST]: (logit, token)
     int* count;                      // [rows]: entries that were to be written
     float* limit;                    // [rows]: the bound, and
-    int* limit_index;                // [rows] the sampled token that set it
+    int* limit_index;                // [rows] the token behind the sampled one that set it
 };
 
 // The sample: logits of tokens 0, s, 2 s, .. of a row (n of them, ld apart). One CTA a row.
@@ -161,22 +162,20 @@ sample_kernel(const float* __restrict__ logits, long long ld, int n, int every, 
     }
     __syncthreads();
     rank<NT>(list, top);
-    if (tid < top) {
+    if (tid == top - 1) {
         const unsigned long long entry = entry_s[tid];
-        out.list[r * LIST + tid] = entry_of(order_in(entry), index_in(entry) * every);
-        if (tid == top - 1) {
-            const bool number = order_in(entry) > 1u;
-            out.limit[r] = number ? value_of(order_in(entry)) : INFINITY;
-            out.limit_index[r] = index_in(entry) * every;
-            out.count[r] = number ? top : LIST + 1;               // (fewer numbers than `top` in the sample: the row is done again)
-        }
+        const float value = value_of(order_in(entry));
+        const bool number = order_in(entry) > 1u;
+        out.limit[r] = number ? value * (value > 0.f ? 1.f - 0x1p-16f : 1.f + 0x1p-16f) : INFINITY;
+        out.limit_index[r] = index_in(entry) * every + 1;
+        out.count[r] = number ? 0 : LIST + 1;                     // (fewer numbers than `top` in the sample: the row is done again)
     }
 }
 
 template <bool TOP>
 __global__ void __launch_bounds__(HEAD_THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const int* __restrict__ targets, int M, int N,
-               int K, int strips, int tiles_per_strip, int every, Scratch out, int* __restrict__ status) {
+               int K, int strips, int tiles_per_strip, Scratch out, int* __restrict__ status) {
     constexpr int STAGES = stages<TOP>();
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -399,7 +398,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
 // One CTA a row. x / table: for a row whose list did not hold all.
 __global__ void __launch_bounds__(NT)
-join_kernel(const int* __restrict__ targets, int V, int strips, int top, int every, Scratch in, Results out, const __nv_bfloat16* __restrict__ x, long long x_stride,
+join_kernel(const int* __restrict__ targets, int V, int strips, int top, Scratch in, Results out, const __nv_bfloat16* __restrict__ x, long long x_stride,
             const __nv_bfloat16* __restrict__ table, long long table_stride, int K, int* __restrict__ status) {
     __shared__ unsigned long long entry_s[CAPACITY], kept_s[MOST_TOP];
     __shared__ uint32_t group_s[GROUPS], limit_s, bound_s;
@@ -415,13 +414,12 @@ join_kernel(const int* __restrict__ targets, int V, int strips, int top, int eve
     const List list = {entry_s, kept_s, &count_s, &limit_s, group_s, &bound_s};
     if (top) {
         const int count = in.count[r];
-        if (tid == 0) { count_s = count <= LIST ? count : 0; limit_s = 0; }
-        if (count <= LIST) {
-            // (sampled tokens came once from the sample, and stand in front, and once more from the product)
+        const bool whole = count >= top && count <= LIST;
+        if (tid == 0) { count_s = whole ? count : 0; limit_s = 0; }
+        if (whole) {
             for (int i = tid; i < count; i += NT) {
                 const unsigned long long entry = in.list[r * LIST + i];
-                if (i < top) entry_s[i] = entry;
-                else entry_s[i] = (int)(uint32_t)entry % every == 0 ? 0ull : entry_of(order_of(__uint_as_float((uint32_t)(entry >> 32))), (int)(uint32_t)entry);
+                entry_s[i] = entry_of(order_of(__uint_as_float((uint32_t)(entry >> 32))), (int)(uint32_t)entry);
             }
             __syncthreads();
             rank<NT>(list, top);
@@ -552,8 +550,8 @@ PS_EXPORT int ps_head_logprobs(const void* x, long long x_stride, const void* ta
     const size_t smem = top ? smem_bytes<true>() : smem_bytes<false>();
     if (!ps::ensure_dynamic_smem((const void*)kernel, smem, raised[top ? 1 : 0])) return PS_ERR_LAUNCH;
     int rc = ps::launch_pdl_clusters(kernel, dim3(2 * pairs), dim3(HEAD_THREADS), smem, s, dim3(2, 1, 1), map_x, map_w, targets, rows, V, K, strips,
-                                     (tiles_n + strips - 1) / strips, every, scratch, status);
+                                     (tiles_n + strips - 1) / strips, scratch, status);
     if (rc) return rc;
-    return ps::launch_pdl(join_kernel, dim3(rows), dim3(NT), 0, s, targets, V, strips, top, every, scratch, out, (const __nv_bfloat16*)x, x_stride,
+    return ps::launch_pdl(join_kernel, dim3(rows), dim3(NT), 0, s, targets, V, strips, top, scratch, out, (const __nv_bfloat16*)x, x_stride,
                           (const __nv_bfloat16*)table, table_stride, K, status);
 }

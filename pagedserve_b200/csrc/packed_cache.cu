@@ -154,12 +154,12 @@ append_kernel(const T* __restrict__ k_src, long long k_stride, const T* __restri
 
 // A position's words (k or v, head, place in the row) over the threads of a CTA, blockIdx.x = position, blockIdx.y = item; out: pages
 // [n_items * span / out_page, 2, kv heads, out_page, head_dim], item i's position p in page i * span / out_page + p / out_page. Positions from kv_len on
-// are left as they are.
+// are left as they are; those without a page, too, or (`fill`) become zeros.
 template <typename T>
 __global__ void __launch_bounds__(256)
 unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
               const int* __restrict__ kv_len, const int* __restrict__ item_row, Pages pages, int span, T* __restrict__ out, int out_log2,
-              int n_kv_heads, int head_dim, int aligned) {
+              int n_kv_heads, int head_dim, int aligned, int fill) {
     pdl_prologue();
     k_pool = pdl_fresh(k_pool);
     v_pool = pdl_fresh(v_pool);
@@ -167,15 +167,18 @@ unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __r
     const int item = blockIdx.y, p = blockIdx.x;
     if (p >= kv_len[item]) return;
     const int page = pages.of(item_row ? item_row[item] : item, p);
-    if (page < 0) return;
+    if (page < 0 && !fill) return;
     const int page_size = 1 << pages.page_log2, row = p & (page_size - 1), out_size = 1 << out_log2;
     const long long out_page = (long long)item * (span >> out_log2) + (p >> out_log2);
     for (int index = threadIdx.x; index < per_row; index += blockDim.x) {
         const int both = index / words, place = index - both * words, plane = both >= n_kv_heads ? 1 : 0, head = both - plane * n_kv_heads;
         const int part = place / groups, j = place - part * groups, d = j * GROUP + part * 8;
-        const unsigned char* slab = (plane ? v_pool : k_pool) + (long long)page * page_stride + (long long)head * slab_bytes(page_size, head_dim);
-        const uint32_t word = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
-        const uint32_t scale = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
+        uint32_t word = 0, scale = 0;
+        if (page >= 0) {
+            const unsigned char* slab = (plane ? v_pool : k_pool) + (long long)page * page_stride + (long long)head * slab_bytes(page_size, head_dim);
+            word = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
+            scale = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
+        }
         const float step = step_of(scale), low = low_of(scale);
         float x[8];
 #pragma unroll
@@ -208,14 +211,14 @@ int append(const void* k_src, long long k_stride, const void* v_src, long long v
 
 template <typename T>
 int unpack(const void* k_pool, const void* v_pool, long long page_stride, const int* kv_len, const int* item_row, const Pages& pages, int n_items,
-           int span, void* out, int out_page, int n_kv_heads, int head_dim, cudaStream_t s) {
+           int span, void* out, int out_page, int n_kv_heads, int head_dim, int fill, cudaStream_t s) {
     const long long words = (long long)2 * n_kv_heads * groups_of(head_dim) * 4;
     const int threads = words >= 256 ? 256 : (int)((words + 31) / 32 * 32);
     if (words > 0x7fffffff) return PS_ERR_UNSUPPORTED;
     const int aligned = !((uintptr_t)out & 15) && head_dim % 8 == 0;
     return launch_pdl(unpack_kernel<T>, dim3(span, n_items), dim3(threads), 0, s, (const unsigned char*)k_pool,
                       (const unsigned char*)v_pool, page_stride, kv_len, item_row, pages, span, (T*)out, log2_of(out_page), n_kv_heads, head_dim,
-                      aligned);
+                      aligned, fill);
 }
 
 }  // namespace packed
@@ -241,10 +244,10 @@ PS_EXPORT int ps_kv_append_packed(const void* k_src, long long k_stride, const v
     return PS_ERR_UNSUPPORTED;
 }
 
-// kv_len / item_row: of the n_items items; span: positions that an item has room for in `out`, a multiple of out_page.
+// kv_len / item_row: of the n_items items; span: positions that an item has room for in `out`, a multiple of out_page; fill: zeros where there is no page.
 PS_EXPORT int ps_kv_unpack(const void* k_pool, const void* v_pool, int n_pages, long long page_stride, const int* kv_len, const int* block_table,
                            int bt_stride, const int* item_row, int n_items, int span, void* out, int out_page, int n_kv_heads, int head_dim,
-                           int page_size, int dtype, void* stream) {
+                           int page_size, int dtype, int fill, void* stream) {
     using namespace ps::packed;
     if (n_items <= 0 || span <= 0) return PS_OK;
     if (!k_pool || !v_pool || !kv_len || !block_table || !out) return PS_ERR_BAD_ARGUMENT;
@@ -253,10 +256,10 @@ PS_EXPORT int ps_kv_unpack(const void* k_pool, const void* v_pool, int n_pages, 
     if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
     const Pages pages = {block_table, bt_stride, n_pages, log2_of(page_size)};
     if (dtype == PS_F32)
-        return unpack<float>(k_pool, v_pool, page_stride, kv_len, item_row, pages, n_items, span, out, out_page, n_kv_heads, head_dim,
+        return unpack<float>(k_pool, v_pool, page_stride, kv_len, item_row, pages, n_items, span, out, out_page, n_kv_heads, head_dim, fill,
                              (cudaStream_t)stream);
     if (dtype == PS_BF16)
-        return unpack<__nv_bfloat16>(k_pool, v_pool, page_stride, kv_len, item_row, pages, n_items, span, out, out_page, n_kv_heads, head_dim,
+        return unpack<__nv_bfloat16>(k_pool, v_pool, page_stride, kv_len, item_row, pages, n_items, span, out, out_page, n_kv_heads, head_dim, fill,
                                      (cudaStream_t)stream);
     return PS_ERR_UNSUPPORTED;
 }

@@ -24,6 +24,7 @@ COLUMN_FACTOR = 2             # in a product's ``accumulate``: its vector multip
 _ACT_CODE = {None: 0, "none": 0, "gelu_tanh": 1, "gelu_erf": 2, "relu_squared": 3, "silu": 4, "tanh": 5}
 PACKED_GROUP, PACKED_MAX_HEAD = 32, 256       # of a cache held in 4 bits: numbers that share a scale; the largest head
 MOST_ALTERNATIVES = 32        # most likely tokens that ``token_logprobs`` gives
+MOST_COUNT = 2 ** 31 - 2 ** 16                # rows or columns that a kernel counts in 32 bits, and a tile beyond them
 _STATUS = {1: "bad argument", 2: "unsupported size or dtype", 3: "kernel launch failed"}
 
 _c_void_p = ctypes.c_void_p
@@ -135,7 +136,7 @@ _SIGNATURES = {
     },
     "packed": {
         "ps_kv_append_packed": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P],
-        "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P],
+        "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
         "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P],
@@ -313,7 +314,7 @@ class Ops:
         self._counters = None        # zeroed int32 scratch of the split attention kernel
         self.launches = 0            # count of kernel launches issued through this object
         self.arena = None            # a StepArena once a runner has attached one: see ``empty``
-        self._ramps = {}             # device -> int32 0, 1, 2, ... (see ``_counting``)
+        self._ramps = {}             # (device, stream) -> int32 0, 1, 2, ... (see ``_counting``)
 
     def empty(self, shape, dtype, device):
         """An uninitialised tensor that lives until the next step begins (from the step arena if a runner
@@ -1229,8 +1230,11 @@ class Ops:
             raise KernelError(f"{what}: a tensor is on {tensor.device}, which is not the current device")
 
     def _packed_rows(self, what, name, rows, count, width, device, dtypes):
-        if not (rows.ndim == 2 and rows.shape == (count, width) and rows.stride(1) == 1 and rows.dtype in dtypes and rows.get_device() == device):
+        if not (rows.ndim == 2 and rows.shape == (count, width) and rows.stride(1) == 1 and rows.dtype in dtypes and rows.get_device() == device
+                and count <= MOST_COUNT):
             _require(rows, name)
+            if count > MOST_COUNT:
+                raise KernelError(f"{what}: up to {MOST_COUNT} rows")
             self._on_current_device(what, rows)
             raise KernelError(f"{what}: {name} must be {count} rows of {width} numbers in {' or '.join(map(str, dtypes))}")
 
@@ -1239,7 +1243,7 @@ class Ops:
         """Round this step's K/V rows ([T, n_kv_heads * head_dim] views of the compute type) to 4 bits and write them into their pages:
         what :meth:`kv_append` is for a cache of the compute type.  ``k_pool`` / ``v_pool`` uint8 [pages, n_kv_heads, slab]
         (:func:`packed_slab_bytes`), ``page_stride`` in bytes.  Token t goes to row ``token_row[t]`` of ``block_table``; one with a
-        position below 0 or without a page is left out.  ``k_src`` or ``v_src`` None leaves that plane as it is."""
+        position below 0 or without a page is left out, and no two go to one place (what it holds then is neither's).  ``k_src`` or ``v_src`` None leaves that plane as it is."""
         what = "kv_append_packed"
         given = [(name, src) for name, src in (("k", k_src), ("v", v_src)) if src is not None]
         if not given:
@@ -1257,10 +1261,10 @@ class Ops:
             n_kv_heads, head_dim, page_size, self.code, _stream()), what)
 
     def kv_unpack(self, k_pool, v_pool, page_stride, kv_len, block_table, item_row, first_item, n_items, span, out, n_kv_heads, head_dim,
-                  page_size):
+                  page_size, fill=False):
         """What a packed cache holds of items ``first_item ..``, as pages of the compute type: ``out`` [n_items * span / P, 2, n_kv_heads, P,
         head_dim], contiguous, P a power of two that divides ``span``.  Position p of the i-th of these items goes to page i * span / P +
-        p / P; positions from ``kv_len`` of the item (or ``span``) on are left as they are.  ``item_row``: the block-table row of each item."""
+        p / P; positions from ``kv_len`` of the item (or ``span``) on are left as they are, those without a page, too, or (``fill``) become zeros.  ``item_row``: the block-table row of each item."""
         what = "kv_unpack"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         _require(out, "out", self.dtype)
@@ -1275,7 +1279,8 @@ class Ops:
         self.launches += 1
         _check(self._packed_library().ps_kv_unpack(
             _ptr(k_pool), _ptr(v_pool), n_pages, page_stride, _ptr(kv_len) + 4 * first_item, _ptr(block_table), block_table.shape[1],
-            _ptr(item_row) + 4 * first_item, n_items, span, _ptr(out), out.shape[3], n_kv_heads, head_dim, page_size, self.code, _stream()), what)
+            _ptr(item_row) + 4 * first_item, n_items, span, _ptr(out), out.shape[3], n_kv_heads, head_dim, page_size, self.code, int(bool(fill)),
+            _stream()), what)
         return out
 
     def _packed_queries(self, what, q, out, n_heads, n_kv_heads, head_dim, scale, softcap, sink, device):
@@ -1337,18 +1342,22 @@ class Ops:
     UNPACKED_BYTES = 512 << 20        # most scratch that prompts take whose rows are unpacked first (but one item's rows always)
 
     def _counting(self, count, device):
-        """int32 0, 1, 2, ...: at least ``count`` of them.  (Never written again, and kept: captured graphs may read it.)"""
-        kept = self._ramps.setdefault(device, [])
-        if not kept or kept[-1].numel() < count:
-            kept.append(torch.arange(max(4096, 2 * count), dtype=torch.int32, device=device))
-        return kept[-1]
+        """int32 0, 1, 2, ...: at least ``count`` of them, kept for the stream that made them.  A graph under capture gets numbers of its own:
+        what it records is not there before it is replayed."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.arange(count, dtype=torch.int32, device=device)
+        stream = _stream()
+        kept = self._ramps.get((device, stream))
+        if kept is None or kept.numel() < count:
+            kept = self._ramps[device, stream] = torch.arange(max(4096, 2 * count), dtype=torch.int32, device=device)
+        return kept
 
     def packed_attention_prompts(self, q, out, k_pool, v_pool, page_stride, q_start, kv_len, block_table, item_row, first_item, n_items,
                                  max_blocks, max_kv_len, n_heads, n_kv_heads, head_dim, page_size, window, scale, softcap=None, sink=None):
         """Causal attention of prompt portions over a packed cache: items ``first_item ..`` of the step, ``max_blocks`` >= the number of 64-query
         blocks they make up, ``max_kv_len`` >= their contexts.  ``q`` / ``out`` are the step's flat token arrays; item i's tokens are rows
-        ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  Otherwise as
-        :meth:`prefill_attention`."""
+        ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  A key without a page is
+        not seen in bfloat16 and is one of zeros in float32, as it is over pages of the compute type.  Otherwise as :meth:`prefill_attention`."""
         what = "packed_attention_prompts"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
@@ -1381,7 +1390,8 @@ class Ops:
         table = counting[:at_once * (span // page)].view(at_once, span // page)
         for start in range(first_item, first_item + n_items, at_once):
             count = min(at_once, first_item + n_items - start)
-            self.kv_unpack(k_pool, v_pool, page_stride, kv_len, block_table, item_row, start, count, span, scratch, n_kv_heads, head_dim, page_size)
+            self.kv_unpack(k_pool, v_pool, page_stride, kv_len, block_table, item_row, start, count, span, scratch, n_kv_heads, head_dim, page_size,
+                           fill=True)
             self._prompts_from_pages(q, out, scratch, q_start[start:], kv_len[start:], table, counting, count, max_blocks, n_heads, n_kv_heads,
                                      head_dim, page, window, scale, softcap, sink)
         return out
@@ -2290,13 +2300,23 @@ class Ops:
         return inner
 
     # ------------------------------------------------------------------ sampling
-    def _logprob_results(self, what, rows, vocabulary, targets, top, device):
+    def _logprob_results(self, what, rows, vocabulary, targets, top, device, results=None):
+        """Checks what the log probabilities' entry points share; the tensors that take the results."""
+        if max(rows, vocabulary) > MOST_COUNT:
+            raise KernelError(f"{what}: rows and vocabularies of up to {MOST_COUNT}")
         _require(targets, "targets", torch.int32)
         if targets.ndim != 1 or targets.numel() != rows or not targets.is_contiguous() or targets.device != device:
             raise KernelError(f"{what}: one int32 token per row, on the device of the rows")
         if not (0 <= top <= min(vocabulary, MOST_ALTERNATIVES)):
             raise KernelError(f"{what}: top is 0 to {MOST_ALTERNATIVES}, and at most the vocabulary")
         self._on_current_device(what, targets)
+        if results is not None:
+            for name, shape, dtype in (("logprob", (rows,), torch.float32), ("entropy", (rows,), torch.float32),
+                                       ("top_logprobs", (rows, top), torch.float32), ("top_ids", (rows, top), torch.int32)):
+                tensor = getattr(results, name)
+                if tensor.shape != shape or tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.device != device:
+                    raise KernelError(f"{what}: results.{name} must be contiguous {shape} in {dtype}, on the device of the rows")
+            return results
         numbers = torch.empty((2 + top, rows), dtype=torch.float32, device=device)
         return TokenLogprobs(numbers[0], numbers[1], numbers[2:].view(rows, top), targets.new_empty((rows, top)))
 
@@ -2304,13 +2324,14 @@ class Ops:
         """:class:`TokenLogprobs` of float32 ``logits`` [rows, vocabulary] and one token a row (int32): its log probability under the row's softmax,
         the distribution's entropy, and the ``top`` largest log probabilities with their tokens (of equal logits the lower token first).
         A token of -1 is none: its log probability is 0.  A token outside the vocabulary sets the status flag and gives NaN.
-        -infinity is a token of probability 0; a NaN or +infinity in a row makes the row's numbers NaN.  ``results``: tensors to write to."""
+        -infinity is a token of probability 0; a NaN or +infinity in a row makes the row's numbers NaN.  ``results``: tensors to write to,
+        contiguous and of these shapes."""
         what = "token_logprobs"
         _require(logits, "logits", torch.float32)
         if logits.ndim != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
             raise KernelError(f"{what}: logits must be rows of a vocabulary")
         rows, V = logits.shape
-        results = results or self._logprob_results(what, rows, V, targets, top, logits.device)
+        results = self._logprob_results(what, rows, V, targets, top, logits.device, results)
         if rows == 0:
             return results
         ld = logits.stride(0) if rows > 1 else V

@@ -130,6 +130,25 @@ def test_heads_that_fool_a_sample(kind, rows):
     check(found, logits, targets, top)
 
 
+@pytest.mark.parametrize("rows,width,V", [(96, 768, 20000), (300, 200, 9000), (1500, 1600, 8500)])
+def test_tokens_with_the_same_row_of_the_table(rows, width, V):
+    """Equal logits whose sums are rounded: the lower tokens, in order, whichever of them a sample of the vocabulary holds."""
+    ops, kinds, top = ops_for(torch.bfloat16), 97, 32
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn(rows, width, generator=g, device=DEV).bfloat16()
+    base = (torch.randn(kinds, width, generator=g, device=DEV) / 4).bfloat16()
+    table = base[torch.arange(V, device=DEV) % kinds].contiguous()
+    found = ops.head_logprobs(x, table, torch.zeros(rows, dtype=torch.int32, device=DEV), top)
+    logits = x.double() @ base.double().t()
+    two, order = logits.topk(2, dim=1)
+    # float32 sums of `width` products are off by at most width * 2^-24 of the products' sizes: beyond that the best kind is a fact
+    clear = two[:, 0] - two[:, 1] > 2 * width * 2.0 ** -24 * (x.double().abs() @ base.double().abs().t()).amax(1)
+    assert clear.sum() > rows * 0.9
+    want = order[:, :1] + kinds * torch.arange(top, device=DEV)
+    assert torch.equal(found.top_ids[clear].long(), want[clear])
+    assert (found.top_logprobs == found.top_logprobs[:, :1])[clear].all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_captured_head(dtype):
     """Captured on a side stream and replayed with other rows."""
@@ -170,6 +189,14 @@ def test_refusals():
                       (torch.zeros(3, 8, device=DEV), table, targets[:1]), (torch.zeros(3, 8, device=DEV), table.t(), targets)):
         with pytest.raises(KernelError):
             ops.head_logprobs(*arguments)
+    good = ops.token_logprobs(logits, targets, 2)
+    assert ops.token_logprobs(logits, targets, 2, results=good) is good
+    for change in (dict(logprob=good.logprob[:2]), dict(entropy=good.entropy.double()), dict(top_logprobs=good.top_logprobs[:, :1]),
+                   dict(top_ids=good.top_ids.long()), dict(top_ids=good.top_ids.t().contiguous().t()), dict(logprob=good.logprob.cpu())):
+        with pytest.raises(KernelError):
+            ops.token_logprobs(logits, targets, 2, results=good._replace(**change))
+    with pytest.raises(KernelError):
+        ops.token_logprobs(logits, targets.long(), 2, results=good)
     empty = ops.token_logprobs(logits[:0], targets[:0], 5)
     assert empty.logprob.shape == (0,) and empty.top_ids.shape == (0, 5)
     assert ops.head_logprobs(torch.zeros(0, 8, device=DEV), table, targets[:0]).entropy.shape == (0,)

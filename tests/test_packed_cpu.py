@@ -79,3 +79,31 @@ def test_tensors_on_the_host_are_refused():
         ops.token_logprobs(torch.zeros(2, 10), torch.zeros(2, dtype=torch.int32))
     with pytest.raises(KernelError, match="CUDA device"):
         ops.head_logprobs(torch.zeros(2, 8), torch.zeros(10, 8), torch.zeros(2, dtype=torch.int32))
+
+
+def test_counts_beyond_32_bits_are_refused():
+    """(kernels count rows and columns in 32 bits: a larger number would be cut without a word)"""
+    from pagedserve_b200.kernels.ops import KernelError, Ops
+
+    ops, targets = Ops(torch.float32), torch.zeros(1, dtype=torch.int32)
+    for rows, vocabulary in ((2 ** 31 - 1, 10), (1, 2 ** 31 - 1), (1, 2 ** 32 + 5)):
+        with pytest.raises(KernelError, match="of up to"):
+            ops._logprob_results("token_logprobs", rows, vocabulary, targets, 0, targets.device)
+
+
+def test_declared_arguments_are_the_sources():
+    """(a call whose declaration is one argument short passes a number where a stream is meant)"""
+    import ctypes
+    import re
+    from pathlib import Path
+
+    from pagedserve_b200.kernels import build, ops
+
+    declared = ops._SIGNATURES["packed"]
+    kinds = {ctypes.c_void_p: "P", ctypes.c_int: "I", ctypes.c_longlong: "L", ctypes.c_float: "F"}
+    found = {}
+    for name in build.LIBRARIES["packed"]:
+        text = (Path(build.__file__).parent.parent / "csrc" / name).read_text()
+        for entry in re.finditer(r"PS_EXPORT int (\w+)\(([^)]*)\)", text):
+            found[entry[1]] = "".join("P" if "*" in part else "L" if "long long" in part else "F" if "float" in part else "I" for part in entry[2].split(","))
+    assert found == {name: "".join(kinds[kind] for kind in arguments) for name, arguments in declared.items()}

@@ -403,6 +403,51 @@ def test_a_captured_step(dtype):
     del graph
 
 
+def test_pages_that_are_missing_may_unpack_as_zeros():
+    ops, heads, dim, page, length = ops_for(F32), 2, 64, 16, 160
+    case = PackedCase([length], heads, dim, page, F32, seed=6)
+    _, planes = on_device(case)
+    table = case.table.clone()
+    table[0, 2], table[0, 5] = -1, case.pages
+    out = torch.full((3, 2, heads, 64, dim), 7.0, device=DEV)
+    ops.kv_unpack(*planes, ints([length]), table.to(DEV), ints([0]), 0, 1, 192, out, heads, dim, page, fill=True)
+    place = torch.arange(192)
+    gone = (place // page == 2) | (place // page == 5)
+    for plane, rows in enumerate(case.held()):
+        flat = out[:, plane].transpose(1, 2).flatten(0, 1).cpu()
+        want = torch.full((192, heads, dim), 7.0)
+        want[:length] = case.context(0, rows)[:length].float()
+        want[gone] = 0.0
+        assert torch.equal(flat, want)
+
+
+def test_prompts_in_float32_first_met_under_capture():
+    """What a captured call needs is its own: an eager call on another stream, before and after the graph is replayed, does not read it."""
+    ops, heads, dim, page, length = ops_for(F32), 2, 64, 16, 150
+    case = PackedCase([length], heads, dim, page, F32, seed=4)
+    _, planes = on_device(case)
+    q = torch.randn(length, heads * dim, generator=torch.Generator().manual_seed(5)).to(DEV)
+    arguments = (ints([0, length]), ints([length]), case.table.to(DEV), ints([0]), 0, 1, 3, length, heads, heads, dim, page, None, 0.125)
+    run = lambda into: ops.packed_attention_prompts(q, into, *planes, *arguments)
+    first, second, third = (torch.zeros_like(q) for _ in range(3))
+    ops._tc_library(), ops._packed_library(), ops.status_flag(q.device)
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        run(first)
+        graph.capture_end()
+    assert ops._ramps == {}
+    with torch.cuda.stream(other):
+        run(second)
+    run(third)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, second) and torch.equal(first, third) and first.abs().sum() > 0
+    del graph
+
+
 def test_refusals_on_the_device():
     from pagedserve_b200.kernels.ops import KernelError
 
