@@ -166,6 +166,7 @@ struct Layout {
     static constexpr int KV_STAGES = 2, KCH = HD / 64, Q_BYTES = BQ * HD * 2, KV_BYTES = BKEY * HD * 2, STAGE_BYTES = 2 * KV_BYTES;
     // two query tiles, the stages, barriers (256 bytes), the rows' factors, then a few words
     static constexpr size_t SMEM = 2 * Q_BYTES + (size_t)KV_STAGES * STAGE_BYTES + 1024 + 256 + 2 * BQ * 4 + 16;
+    static constexpr int PART_ROW = HD + 4;                         // pitch of a share's O rows: eight neighbouring rows on eight groups of four banks
     // TMEM: scores of either tile (P takes their place), then O of either
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
 };
@@ -272,19 +273,21 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         block -= blocks;
     }
     if (item < 0) return;
-    const int h = blockIdx.x, g = h / (n_heads / n_kv_heads);
+    const int h = blockIdx.x, g = h / (n_heads / n_kv_heads), share = blockIdx.z, shares = gridDim.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int qs = q_start[item], q_len = q_start[item + 1] - qs;
     const int pos0 = kv_len[item] - q_len + qb * 2 * BQ;              // position of the block's first query
     const int rows = min(2 * BQ, q_len - qb * 2 * BQ), tok0 = qs + qb * 2 * BQ;
     const int hi = pos0 + rows - 1, lo = pos0 < 0 ? 0 : first_visible_key(pos0, window);
-    const int kb_first = lo / BKEY, kb_last = max(hi, 0) / BKEY;
-    // the key tiles that a query tile's rows see (a second tile without rows: none)
+    // the share's run of the block's key tiles
+    const int kb_all = lo / BKEY, kb_count = max(hi, 0) / BKEY - kb_all + 1;
+    const int kb_first = kb_all + kb_count * share / shares, kb_last = kb_all + kb_count * (share + 1) / shares - 1;
+    // those of them that a query tile's rows see (a second tile without rows: none)
     auto first_of = [&](int x) {
         const int p = pos0 + x * BQ;
-        return x * BQ >= rows ? kb_last + 1 : (p < 0 ? 0 : first_visible_key(p, window)) / BKEY;
+        return x * BQ >= rows ? kb_last + 1 : max(kb_first, (p < 0 ? 0 : first_visible_key(p, window)) / BKEY);
     };
-    auto last_of = [&](int x) { return max(pos0 + min(rows, (x + 1) * BQ) - 1, 0) / BKEY; };
+    auto last_of = [&](int x) { return min(kb_last, max(pos0 + min(rows, (x + 1) * BQ) - 1, 0) / BKEY); };
     const int table_row = item_row ? item_row[item] : item;
     const int page_size = 1 << cache.pages.page_log2, groups = groups_of(head_dim);
     const long long head_at = (long long)g * slab_bytes(page_size, head_dim);
@@ -315,6 +318,33 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // eight numbers of a query row's result, from d on
+    auto store8 = [&](int place, int d, const float (&v)[8]) {
+        const long long to = (long long)(tok0 + place) * out_stride + (long long)h * head_dim + d;
+        if (aligned_out && d + 8 <= head_dim) {
+            if (extras.wide) {
+                float4* at = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to);
+                at[0] = make_float4(v[0], v[1], v[2], v[3]);
+                at[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                uint4 pack;
+                uint32_t* two = reinterpret_cast<uint32_t*>(&pack);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                    two[i] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + to) = pack;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d + i < head_dim) store_result(reinterpret_cast<__nv_bfloat16*>(out), to + i, v[i], extras);
+        }
+    };
+    // what a share leaves of its rows, over the tiles: O, then the bases and the sums of the weights
+    float* part_s = reinterpret_cast<float*>(base);
+    float *part_m = part_s + 2 * BQ * L::PART_ROW, *part_l = part_m + 2 * BQ;
 
     if (warp < 4) {
         // ------------------------------------------------ makers: thread r has key r of every tile and its value, and row r of both query tiles
@@ -517,7 +547,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         const uint32_t s_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::S_COL + x * 128;
         const uint32_t o_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::O_COL + x * HD;
         float base_m = 0.f, limit = -INFINITY, l_run = 0.f;        // in log2 units: the base of the weights, what a score may reach
-        if (extras.sink && extras.sink[h] != -INFINITY) {
+        if (share == 0 && extras.sink && extras.sink[h] != -INFINITY) {
             base_m = extras.sink[h] * 1.4426950408889634f;
             limit = base_m + HEADROOM;
             l_run = 1.f;
@@ -599,42 +629,37 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             mbar_arrive(&p_ready[2 * x + half]);
         }
         if (ok && !mbar_wait(&o_full[x], 0, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 61); }
-        if (ok) {
-            tc_fence_after();
-            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-            const long long to = (long long)(tok0 + place) * out_stride + (long long)h * head_dim;
+        tc_fence_after();
+        if (shares > 1) {
+            // (every row has waited for its O: no product reads the tiles any more, and what the makers made is all taken; but for the queries
+            // of a share without keys)
+            if (!mbar_wait(&q_full[1], 0, abort_flag) && lane == 0) atomicExch(status, 62);
+            asm volatile("bar.sync 1, %0;" ::"n"(2 * BQ) : "memory");
+            part_m[place] = limit > -INFINITY ? base_m : -INFINITY;
+            part_l[place] = l_run;
+        }
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-                uint32_t orr[16];
+        for (int c = 0; c < HD; c += 16) {
+            uint32_t orr[16];
+            if (ok) {
                 tmem_ld16(o_at + c, orr);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (place < rows) {
+            } else {
 #pragma unroll
-                    for (int d = 0; d < 16; d += 8) {
-                        float v[8];
+                for (int i = 0; i < 16; ++i) orr[i] = 0u;          // (the share has no key that the tile sees)
+            }
+            if (shares > 1) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(orr[d + i]) * inv;
-                        if (aligned_out && c + d + 8 <= head_dim) {
-                            if (extras.wide) {
-                                float4* at = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to + c + d);
-                                at[0] = make_float4(v[0], v[1], v[2], v[3]);
-                                at[1] = make_float4(v[4], v[5], v[6], v[7]);
-                            } else {
-                                uint4 pack;
-                                uint32_t* two = reinterpret_cast<uint32_t*>(&pack);
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<uint4*>(part_s + place * L::PART_ROW + c + i) = make_uint4(orr[i], orr[i + 1], orr[i + 2], orr[i + 3]);
+            } else if (ok && place < rows) {
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                                    two[i] = *reinterpret_cast<const uint32_t*>(&b);
-                                }
-                                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + to + c + d) = pack;
-                            }
-                        } else {
+                for (int d = 0; d < 16; d += 8) {
+                    float v[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (c + d + i < head_dim) store_result(reinterpret_cast<__nv_bfloat16*>(out), to + c + d + i, v[i], extras);
-                        }
-                    }
+                    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(orr[d + i]) * inv;
+                    store8(place, c + d, v);
                 }
             }
         }
@@ -645,22 +670,62 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)L::TMEM_COLS) : "memory");
     }
-    const float k_most = __uint_as_float(sizes_s[0]), v_most = __uint_as_float(sizes_s[1]);
-    if (sizes_s[2] || (k_most > 0.f && k_most < LEAST) || (v_most > 0.f && v_most < LEAST))
+    float k_most = __uint_as_float(sizes_s[0]), v_most = __uint_as_float(sizes_s[1]);
+    uint32_t strange = sizes_s[2];
+    if (shares > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        for (int other = 0; other < shares; ++other) {
+            k_most = fmaxf(k_most, __uint_as_float(ld_cluster_u32(&sizes_s[0], other)));
+            v_most = fmaxf(v_most, __uint_as_float(ld_cluster_u32(&sizes_s[1], other)));
+            strange |= ld_cluster_u32(&sizes_s[2], other);
+        }
+    }
+    if (strange || (k_most > 0.f && k_most < LEAST) || (v_most > 0.f && v_most < LEAST)) {
         rows_again(q, q_stride, out, out_stride, extras.wide, cache, table_row, head_at, h, head_dim, tok0, pos0, rows, window, scale, softcap, extras.sink,
-                   warp, THREADS / 32, lane);
+                   share * (THREADS / 32) + warp, shares * (THREADS / 32), lane);
+    } else if (shares > 1) {
+        // a part of the rows each, eight numbers a thread
+        constexpr int PIECES = HD / 8;
+        const int first = rows * share / shares, count = rows * (share + 1) / shares - first;
+        for (int i = threadIdx.x; i < count * PIECES; i += THREADS) {
+            const int place = first + i / PIECES, d = i % PIECES * 8;
+            if (d >= head_dim) continue;
+            float top = -INFINITY, total = 0.f, v[8];
+            for (int other = 0; other < shares; ++other) top = fmaxf(top, ld_cluster_f32(part_m + place, other));
+            const float ground = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+            for (int other = 0; other < shares; ++other) {
+                const float by = ex2(ld_cluster_f32(part_m + place, other) - ground);
+                const float4 a = ld_cluster_f32x4(part_s + place * L::PART_ROW + d, other), b = ld_cluster_f32x4(part_s + place * L::PART_ROW + d + 4, other);
+                const float one[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                total = fmaf(ld_cluster_f32(part_l + place, other), by, total);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = fmaf(one[j], by, v[j]);
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= inv;
+            store8(place, d, v);
+        }
+    }
+    if (shares > 1) {
+        __syncwarp();
+        cluster_sync_all();                                        // the shares stay until they were read
+    }
 }
 
 template <int HD, bool CAPPED>
 int launch(const void* q, long long q_stride, void* out, long long out_stride, int wide, const Cache& cache, const int* q_start, const int* kv_len,
            const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
-           const float* sink, int* status, cudaStream_t s) {
+           const float* sink, int shares, int* status, cudaStream_t s) {
     auto kernel = prompts_kernel<HD, CAPPED>;
     static size_t raised[MAX_DEVICES] = {0};
     if (!ensure_dynamic_smem((const void*)kernel, Layout<HD>::SMEM, raised)) return PS_ERR_LAUNCH;
     const int aligned_q = !((uintptr_t)q & 15) && q_stride % 8 == 0 && head_dim % 8 == 0;
     const int aligned_out = !((uintptr_t)out & 15) && out_stride % 8 == 0 && head_dim % 8 == 0;
-    return launch_pdl(kernel, dim3(n_heads, max_blocks), dim3(THREADS), Layout<HD>::SMEM, s, (const __nv_bfloat16*)q, q_stride, out, out_stride, cache,
+    return launch_pdl_cluster(kernel, dim3(n_heads, max_blocks, shares), dim3(THREADS), Layout<HD>::SMEM, s, shares, (const __nv_bfloat16*)q, q_stride, out, out_stride, cache,
                       q_start, kv_len, item_row, n_items, n_heads, n_kv_heads, head_dim, window, scale, softcap, softmax_extras(scale, softcap, sink, wide),
                       aligned_q, aligned_out, status);
 }
@@ -670,18 +735,20 @@ int launch(const void* q, long long q_stride, void* out, long long out_stride, i
 
 // q / out: the step's flat rows of n_heads * head_dim numbers; item i's tokens are rows q_start[i] .. q_start[i + 1], the last ones of kv_len[i], its
 // pages row item_row[i] of block_table (bt_stride wide).  max_blocks >= sum over the items of ceil(tokens / 256).  wide: out is float32.
+// shares: CTAs (a cluster) that share a block's keys out, 1, 2, 4 or 8.
 PS_EXPORT int ps_packed_prompts_tc(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
                                    int n_pages, long long page_stride, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
                                    const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int page_size,
-                                   int window, float scale, float softcap, const float* sink, int* status, void* stream) {
+                                   int window, float scale, float softcap, const float* sink, int shares, int* status, void* stream) {
     using namespace ps::packedtc;
     if (n_items <= 0 || max_blocks <= 0) return PS_OK;
     if (!q || !out || !k_pool || !v_pool || !q_start || !kv_len || !block_table || !status) return PS_ERR_BAD_ARGUMENT;
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_blocks > 65535) return PS_ERR_BAD_ARGUMENT;
     if (!ps::packed::sizes_ok(n_kv_heads, head_dim, page_size) || head_dim > 128) return PS_ERR_UNSUPPORTED;
+    if (shares != 1 && shares != 2 && shares != 4 && shares != 8) return PS_ERR_BAD_ARGUMENT;
     if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
     const Cache cache = {(const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, {block_table, bt_stride, n_pages, ps::packed::log2_of(page_size)}};
     auto run = head_dim <= 64 ? (softcap > 0.f ? launch<64, true> : launch<64, false>) : (softcap > 0.f ? launch<128, true> : launch<128, false>);
     return run(q, q_stride, out, out_stride, wide, cache, q_start, kv_len, item_row, n_items, max_blocks, n_heads, n_kv_heads, head_dim, window, scale,
-               softcap, sink, status, (cudaStream_t)stream);
+               softcap, sink, shares, status, (cudaStream_t)stream);
 }

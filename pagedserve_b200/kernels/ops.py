@@ -139,7 +139,7 @@ _SIGNATURES = {
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
-        "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P],
+        "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P, _P],
         "ps_head_logprobs_strips": [_I, _I],
         "ps_head_logprobs": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P],
         "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
@@ -1353,11 +1353,13 @@ class Ops:
         return kept
 
     def packed_attention_prompts(self, q, out, k_pool, v_pool, page_stride, q_start, kv_len, block_table, item_row, first_item, n_items,
-                                 max_blocks, max_kv_len, n_heads, n_kv_heads, head_dim, page_size, window, scale, softcap=None, sink=None):
+                                 max_blocks, max_kv_len, n_heads, n_kv_heads, head_dim, page_size, window, scale, softcap=None, sink=None,
+                                 shares=0):
         """Causal attention of prompt portions over a packed cache: items ``first_item ..`` of the step, ``max_blocks`` >= the number of 64-query
         blocks they make up, ``max_kv_len`` >= their contexts.  ``q`` / ``out`` are the step's flat token arrays; item i's tokens are rows
         ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  A key without a page is
-        not seen in bfloat16 and is one of zeros in float32, as it is over pages of the compute type.  Otherwise as :meth:`prefill_attention`."""
+        not seen in bfloat16 and is one of zeros in float32, as it is over pages of the compute type.  ``shares`` (bfloat16): CTAs for the keys of 256
+        queries, 1, 2, 4 or 8 (0: by the counts).  Otherwise as :meth:`prefill_attention`."""
         what = "packed_attention_prompts"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
@@ -1373,12 +1375,20 @@ class Ops:
             raise KernelError(f"{what}: heads of {head_dim} in {self.dtype} with these strides go token by token (packed_attention_tokens)")
         if self.dtype == torch.bfloat16:
             # (an entry of b blocks of 64 queries has at most (b + 3) / 4 of 256)
+            blocks = (max_blocks + 3 * n_items) // 4
+            if not shares:
+                # Shares pay where they leave every CTA an SM, from two tiles of 128 keys each on (us at 1, 2, 4 shares: 128 queries behind 3,872
+                # keys, 12 heads of 64, 68.4, 41.3, 26.5; 256 behind 744 24.7, 20.7, 17.9; two prompts of 1,024 27.6, 31.1, 51.4).
+                keys = min(int(max_kv_len), abs(window) + 255) if window else int(max_kv_len)
+                shares = 1
+                while shares < 8 and n_heads * blocks * shares * 2 <= 148 and shares * 2 <= keys // 256:
+                    shares *= 2
             self.launches += 1
             _check(self._packed_library().ps_packed_prompts_tc(
                 _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
                 page_stride, _ptr(q_start) + 4 * first_item, _ptr(kv_len) + 4 * first_item, _ptr(block_table), block_table.shape[1],
-                _ptr(item_row) + 4 * first_item, n_items, (max_blocks + 3 * n_items) // 4, n_heads, n_kv_heads, head_dim, page_size, window or 0, scale,
-                float(softcap or 0.0), _ptr(sink), _ptr(self.status_flag(device)), _stream()), what)
+                _ptr(item_row) + 4 * first_item, n_items, blocks, n_heads, n_kv_heads, head_dim, page_size, window or 0, scale,
+                float(softcap or 0.0), _ptr(sink), shares, _ptr(self.status_flag(device)), _stream()), what)
             return out
         # float32: the rows as pages of the compute type, some items at a time, and the kernels for those.
         page = 64

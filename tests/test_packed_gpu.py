@@ -342,6 +342,51 @@ def test_nan_and_missing_pages_in_prompts():
         assert ((got[1, i:i + 1] - want).abs() <= bound_of(want, weighted, sizes, 0.125, BF16, 2.0 ** -10, dim, 2.0 ** -11)).all()
 
 
+@pytest.mark.parametrize("shares", [1, 2, 4, 8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,softcap,with_sink", [(None, None, False), (150, None, True), (None, 3.0, True)])
+def test_shares_of_the_keys_of_a_block(shares, dim, window, softcap, with_sink):
+    """More shares than tiles of keys, shares whose keys a query tile does not see, rows of fewer than a block."""
+    ops, heads, kv_heads, page = ops_for(BF16), 4, 2, 16
+    news, lengths = [300, 5, 129, 1, 256], [1500, 700, 129, 1, 900]
+    case = PackedCase(lengths, kv_heads, dim, page, BF16, seed=9)
+    _, planes = on_device(case)
+    starts = [0]
+    for new in news:
+        starts.append(starts[-1] + new)
+    g = torch.Generator().manual_seed(dim)
+    q = torch.randn(starts[-1], heads * dim, generator=g).bfloat16()
+    sink = torch.randn(heads, generator=g) if with_sink else None
+    out = torch.full((starts[-1] + 3, heads * dim), 7.0, dtype=BF16, device=DEV)
+    ops.packed_attention_prompts(q.to(DEV), out[:-3], *planes, ints(starts), ints(lengths), case.table.to(DEV), ints(range(5)), 0, 5, 5 + 1 + 3 + 1 + 4, 1500,
+                                 heads, kv_heads, dim, page, window, 0.125, softcap=softcap, sink=None if sink is None else sink.to(DEV), shares=shares)
+    assert (out[-3:] == 7.0).all()
+    for i in range(5):
+        k, v = (case.context(i, held_rows) for held_rows in case.held())
+        mine = slice(starts[i], starts[i + 1])
+        positions = torch.arange(lengths[i] - news[i], lengths[i])
+        want, weighted, sizes = attention(q[mine].double().view(-1, heads, dim), k, v, positions, 0.125, window=window, softcap=softcap, sink=sink)
+        got = out[mine].cpu().double().view(-1, heads, dim)
+        assert ((got - want).abs() <= bound_of(want, weighted, sizes, 0.125, BF16, 2.0 ** -10, dim, 2.0 ** -11)).all()
+
+
+def test_shares_and_rows_that_are_formed_again():
+    """A NaN in one share's keys is met by all of them."""
+    ops, heads, dim, page, length = ops_for(BF16), 2, 64, 16, 1100
+    case = PackedCase([length], heads, dim, page, BF16, seed=6)
+    case.v[900, 1, 40] = float("nan")                                   # head 1, second group
+    _, planes = on_device(case)
+    q = torch.randn(300, heads * dim, generator=torch.Generator().manual_seed(3)).bfloat16().to(DEV)
+    arguments = (ints([0, 300]), ints([length]), case.table.to(DEV), ints([0]), 0, 1, 5, length, heads, heads, dim, page, None, 0.125)
+    once = ops.packed_attention_prompts(q, torch.empty_like(q), *planes, *arguments, shares=1)
+    bad = once.view(300, heads, dim).isnan()
+    assert bad[100:, 1, 32:].all() and bad.sum() == 200 * 32            # (queries from position 800 on)
+    for shares in (2, 4, 8):
+        shared = ops.packed_attention_prompts(q, torch.empty_like(q), *planes, *arguments, shares=shares)
+        assert torch.equal(shared.isnan(), once.isnan())
+        assert torch.equal(shared.view(300, heads, dim)[:, 1].nan_to_num(), once.view(300, heads, dim)[:, 1].nan_to_num())
+
+
 def test_prompts_in_several_rounds():
     """Unpacked rows of some items at a time."""
     ops, heads, dim, page = ops_for(F32), 2, 64, 16
