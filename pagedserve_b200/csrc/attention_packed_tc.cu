@@ -1,23 +1,27 @@
 // Causal attention of prompt portions over a cache held in 4 bits on tcgen05 tensor cores (bfloat16 queries, head sizes up to 128; packed.cuh
 // has the cache's format).
 //
-// One CTA per (block of 256 query tokens of one request, head), tiles of 128 keys aligned to absolute positions. The block is two tiles of 128
-// queries that take turns: while the rows of one form their weights, the tensor cores work for the other.
+// One CTA per (block of 256 query tokens of one request, head, share of the keys), tiles of 128 keys aligned to absolute positions. The block is two
+// tiles of 128 queries that take turns: while the rows of one form their weights, the tensor cores work for the other.
 //   warps 0..3   a key and its value a thread: codes and scales come to registers ahead of their tile, become low + code * step (one rounding to float16,
 //                2^-12 of the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact as
-//                its own) and go to the swizzled tile, 16 bytes a word of codes; before that the queries' rows
+//                its own) and go to the swizzled tile, 16 bytes a word of codes
 //   warps 4, 13  issue of S = Q K^T and O += P V for the first and the second query tile (4: TMEM allocation, too)
-//   warps 5..12  softmax, a thread per query row: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves, and O with it, only when
-//                a score is beyond it by 2^8, which float16 has room for
+//   warps 5..12  a thread per query row: the query to its tile, then softmax: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves,
+//                and O with it, only when a score is beyond it by 2^8, which float16 has room for
 // A tile's keys go through in two halves of 64, whose scores have columns of their own: P of a half takes the place of its scores, P V of the half is
-// issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half. Rows hardly wait, then.
+// issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half.
 // Queries are scaled row by row by a power of two, so that any bfloat16 row is one in float16. Keys and values are not: a block that meets one
 // beyond 60,000, or none beyond 2^-9, or a NaN, or a key without a page, forms its rows again in float32 from the codes (rows_again below), which is slow and
 // right.
+// Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each.
 //
-// What bounds it: exponentials, 16 a clock and SM: 2,048 clocks for 256 queries and 128 keys, as long as the products at head size 128.  One tile's scores at a time
-// for a query tile (scores, weights, P V, scores in turn) took 4,700 clocks at head size 64, 2,200 of them the way from P to the next scores; an MMA takes about 70 clocks
-// to issue, so either query tile has a warp for it.
+// What bounds it: per 128 keys and 256 queries the rows' instructions (about 2,500 clocks, 2,048 of them exponentials) at head size 64, the makers' (1,250 for
+// the keys and as much for the values) at 128; and about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
+// codes) and the first passes through everything. Two prompts of 1,024 (12 heads of 64) 25.6 us; three portions of 683 and fewer queries
+// behind up to 8,192 keys (16 heads on 4 of 128) 170 us, 0.62 PFLOP/s. The way there at those two: an MMA issued behind `lane == 0`, or predicated, takes 70 to 97
+// clocks, behind elect.sync 45 (190 -> 182 us at head size 128, one query tile 68 -> 54); the queries by the rows' warps, which wait anyway, instead of the
+// makers (26.8 -> 25.6, 182 -> 170). Two threads a row, 32 scores each, were slower (30 us, 190): a meeting of the two each half, and 80 registers a thread.
 #include <type_traits>
 
 #include "packed.cuh"
@@ -75,24 +79,27 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo_
     desc |= (uint64_t)2 << 61;
     return desc;
 }
-// Issued by the thread of a warp whose `one` is set, while the whole warp comes along: its control flow and descriptors then stay uniform. (Inside a branch
-// that one lane takes, an MMA's operands are moved to uniform registers one by one: 80 clocks an MMA, 960 for a tile's twelve.)
-__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+// one lane of a warp, chosen by the instruction that the compiler knows to choose one (behind `lane == 0` it moves an MMA's operands one by one:
+// 70 to 97 clocks an MMA; in this branch 45, at N = 64)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen != 0;
 }
-__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc) : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint32_t one, uint64_t* bar) {
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(one) : "memory");
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile(
@@ -164,8 +171,8 @@ __device__ __forceinline__ uint4 numbers_of(uint32_t word, uint32_t step, uint32
 template <int HD>
 struct Layout {
     static constexpr int KV_STAGES = 2, KCH = HD / 64, Q_BYTES = BQ * HD * 2, KV_BYTES = BKEY * HD * 2, STAGE_BYTES = 2 * KV_BYTES;
-    // two query tiles, the stages, barriers (256 bytes), the rows' factors, then a few words
-    static constexpr size_t SMEM = 2 * Q_BYTES + (size_t)KV_STAGES * STAGE_BYTES + 1024 + 256 + 2 * BQ * 4 + 16;
+    // two query tiles, the stages, barriers (256 bytes), then a few words
+    static constexpr size_t SMEM = 2 * Q_BYTES + (size_t)KV_STAGES * STAGE_BYTES + 1024 + 256 + 16;
     static constexpr int PART_ROW = HD + 4;                         // pitch of a share's O rows: eight neighbouring rows on eight groups of four banks
     // TMEM: scores of either tile (P takes their place), then O of either
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
@@ -248,7 +255,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     unsigned char* q_s = base;                // two tiles
     unsigned char* kv_s = base + 2 * L::Q_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + (size_t)KV_STAGES * L::STAGE_BYTES);
-    uint64_t* q_full = bars;                  // [2] makers -> MMA and rows
+    uint64_t* q_full = bars;                  // [2] rows -> MMA
     uint64_t* k_full = q_full + 2;            // [KV_STAGES] makers -> MMA
     uint64_t* k_empty = k_full + KV_STAGES;   // [KV_STAGES] MMA -> makers
     uint64_t* v_full = k_empty + KV_STAGES;   // [KV_STAGES] makers -> MMA
@@ -259,8 +266,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     uint64_t* o_full = o_done + 2;            // [2] MMA -> rows: O is complete (o_done could be a phase or two behind where no one waited for it)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* factor_s = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(bars) + 256);      // [2 * BQ] what undoes a query row's scale
-    uint32_t* sizes_s = reinterpret_cast<uint32_t*>(factor_s + 2 * BQ);          // largest key, largest value (bits), whether something is strange
+    uint32_t* sizes_s = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(bars) + 256);      // largest key, largest value (bits), whether something is strange
 
     pdl_prologue();
     q = pdl_fresh(q);
@@ -295,14 +301,14 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < KV_STAGES; ++s) {
-            mbar_init(&k_full[s], MAKERS); mbar_init(&k_empty[s], 2);
-            mbar_init(&v_full[s], MAKERS); mbar_init(&v_empty[s], 2);
+            mbar_init(&k_full[s], MAKERS / 32); mbar_init(&k_empty[s], 2);
+            mbar_init(&v_full[s], MAKERS / 32); mbar_init(&v_empty[s], 2);
         }
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&q_full[x], MAKERS);
+            mbar_init(&q_full[x], BQ / 32);
             for (int half = 0; half < 2; ++half) {
                 mbar_init(&s_full[2 * x + half], 1);
-                mbar_init(&p_ready[2 * x + half], BQ);
+                mbar_init(&p_ready[2 * x + half], BQ / 32);
             }
             mbar_init(&o_done[x], 1);
             mbar_init(&o_full[x], 1);
@@ -318,6 +324,11 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // for a whole warp (arrivals of all its lanes take turns at the barrier: 512 of them a half of a tile cost more than the half's exponentials)
+    auto arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
     // eight numbers of a query row's result, from d on
     auto store8 = [&](int place, int d, const float (&v)[8]) {
         const long long to = (long long)(tok0 + place) * out_stride + (long long)h * head_dim + d;
@@ -347,7 +358,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     float *part_m = part_s + 2 * BQ * L::PART_ROW, *part_l = part_m + 2 * BQ;
 
     if (warp < 4) {
-        // ------------------------------------------------ makers: thread r has key r of every tile and its value, and row r of both query tiles
+        // ------------------------------------------------ makers: thread r has key r of every tile and its value
         const int r = threadIdx.x;
         uint4 k_codes[GROUPS_MOST], v_codes[GROUPS_MOST];
         uint32_t k_scales[GROUPS_MOST], v_scales[GROUPS_MOST];
@@ -403,15 +414,104 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        // (in front of the queries' rows where registers do for both)
         locate(kb_first);
-        if constexpr (HD == 64) {
-            fetch(cache.k_pool, k_codes, k_scales);
-            fetch(cache.v_pool, v_codes, v_scales);
+        fetch(cache.k_pool, k_codes, k_scales);
+        fetch(cache.v_pool, v_codes, v_scales);
+        uint32_t it = 0;
+        for (int kb = kb_first; kb <= kb_last; ++kb, ++it) {
+            const int s = it % KV_STAGES;
+            const uint32_t free = ((it / KV_STAGES) & 1) ^ 1;
+            unsigned char* tile = kv_s + (size_t)s * L::STAGE_BYTES;
+            if (kb < kb_last) locate(kb + 1);
+            if (!mbar_wait(&k_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 51); break; }
+            make(tile, k_codes, k_scales, k_most);
+            arrive(&k_full[s]);
+            if (kb < kb_last) fetch(cache.k_pool, k_codes, k_scales);
+            if (!mbar_wait(&v_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 52); break; }
+            make(tile + L::KV_BYTES, v_codes, v_scales, v_most);
+            arrive(&v_full[s]);
+            if (kb < kb_last) fetch(cache.v_pool, v_codes, v_scales);
         }
+        const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_most)), v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_most));
+        const bool any = __any_sync(0xffffffffu, strange);
+        if (lane == 0) {
+            atomicMax(&sizes_s[0], k_bits);
+            atomicMax(&sizes_s[1], v_bits);
+            if (any) atomicExch(&sizes_s[2], 1u);
+        }
+    } else if (warp == 4 || warp == 13) {
+        // ------------------------------------------------ MMA issuers, one for each query tile
+        // D f32, A/B f16: S = Q K^T both K-major, N = 64; O = P V with A from TMEM and B MN-major (bit 16), N = HD
+        constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        const int x = warp == 4 ? 0 : 1, first = first_of(x), last = last_of(x);
+        const uint32_t s_at = tmem_base + L::S_COL + x * 128, o_at = tmem_base + L::O_COL + x * HD;
+        const uint64_t q_desc = desc_sw128(smem_u32(q_s + x * L::Q_BYTES), 16);
+        auto waits = [&](uint64_t* bar, uint32_t parity, int code) {
+            const bool there = mbar_wait(bar, parity, abort_flag);
+            if (!there) atomicExch(status, code);
+            tc_fence_after();
+            return there;
+        };
+        auto scores = [&](int kb, int half) {                      // (64 rows of a tile are 8,192 bytes)
+            const uint64_t k_desc = desc_sw128(smem_u32(kv_s + (size_t)((kb - kb_first) % KV_STAGES) * L::STAGE_BYTES) + half * 8192, 16);
+#pragma unroll
+            for (int c = 0; c < L::KCH; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_ss(s_at + half * 64, q_desc + c * (BQ * 128 / 16) + 2 * k, k_desc + c * (BKEY * 128 / 16) + 2 * k, idesc_qk, (c | k) ? 1u : 0u);
+            umma_commit(&s_full[2 * x + half]);
+        };
+        if (elect_one()) {
+            bool ok = true;
+            uint32_t taken = 0;                                        // key tiles of this query tile whose weights were taken
+            for (int kb = kb_first - 1; kb <= kb_last && ok; ++kb) {   // weights of tile kb, scores of kb + 1
+                const uint32_t it = (uint32_t)(kb - kb_first);
+                const bool weighs = kb >= first && kb <= last, next = kb + 1 <= kb_last, asks = kb + 1 >= first && kb + 1 <= last;
+                if (next) ok = waits(&k_full[(it + 1) % KV_STAGES], ((it + 1) / KV_STAGES) & 1, 54);
+                if (ok && kb + 1 == first) ok = waits(&q_full[x], 0, 53);
+                if (ok && kb >= kb_first) ok = waits(&v_full[it % KV_STAGES], (it / KV_STAGES) & 1, 57);
 #pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-            const int place = x * BQ + r;
+                for (int half = 0; half < 2 && ok; ++half) {
+                    if (weighs) {
+                        ok = waits(&p_ready[2 * x + half], taken & 1, 56);
+                        if (!ok) break;
+                        const uint64_t v_desc = desc_sw128(smem_u32(kv_s + (size_t)(it % KV_STAGES) * L::STAGE_BYTES) + L::KV_BYTES + half * 8192, BKEY * 128);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)                    // 16 keys = 2,048 bytes of V, 8 columns of P
+                            umma_ts(o_at, s_at + half * 64 + 8 * k, v_desc + (uint64_t)((2048 * k) >> 4), idesc_pv, (taken | (uint32_t)half | (uint32_t)k) ? 1u : 0u);
+                        umma_commit(&o_done[x]);
+                        if (kb == last && half == 1) umma_commit(&o_full[x]);
+                    }
+                    if (asks) scores(kb + 1, half);
+                }
+                if (ok && weighs) ++taken;
+                // (a tile that this query tile does not see is given back as soon as it is there)
+                if (ok && kb >= kb_first) umma_commit(&v_empty[it % KV_STAGES]);
+                if (ok && next) umma_commit(&k_empty[(it + 1) % KV_STAGES]);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------ rows
+        const int quarter = warp & 3, x = (warp - 5) >> 2;
+        const int r = quarter * 32 + lane, place = x * BQ + r, pos = pos0 + place;
+        const int first = first_of(x), last = last_of(x);
+        const int lo_row = pos < 0 ? 0 : first_visible_key(pos, window);
+        const int pos_first = pos0 + x * BQ, pos_last = pos0 + min(rows, (x + 1) * BQ) - 1;
+        const int lo_all = pos_last < 0 ? 0 : first_visible_key(pos_last, window);        // the first key that every row of the tile sees
+        const uint32_t s_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::S_COL + x * 128;
+        const uint32_t o_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::O_COL + x * HD;
+        float base_m = 0.f, limit = -INFINITY, l_run = 0.f;        // in log2 units: the base of the weights, what a score may reach
+        if (share == 0 && extras.sink && extras.sink[h] != -INFINITY) {
+            base_m = extras.sink[h] * 1.4426950408889634f;
+            limit = base_m + HEADROOM;
+            l_run = 1.f;
+        }
+        bool ok = first <= last;
+        // the row's query, scaled by a power of two, to its tile
+        float factor;
+        {
             const __nv_bfloat16* row = q + (long long)(tok0 + place) * q_stride + (long long)h * head_dim;
             float most = 0.f;
             bool odd = false;
@@ -429,16 +529,6 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
                     }
                 }
             }
-            auto each = [&](auto f) {                              // two neighbouring numbers to a word
-#pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    uint32_t v[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = f(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-                    raw[i] = make_uint4(v[0], v[1], v[2], v[3]);
-                }
-            };
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
                 const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -452,109 +542,18 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             // 2^up brings the largest to [256, 512); a NaN or infinity stays one
             const int up = most > 0.f && !odd ? min(126, 135 - max(1, (int)(__float_as_uint(most) >> 23))) : 0;
             const float by = __uint_as_float((uint32_t)(127 + up) << 23);
-            factor_s[place] = __uint_as_float((uint32_t)(127 - up) << 23);
-            each([&](float a, float b) { return half_pair(a * by, b * by); });
+            factor = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<uint4*>(q_s + x * L::Q_BYTES + tile_byte(r, 8 * i)) = raw[i];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&q_full[x]);
-        }
-        if constexpr (HD != 64) {
-            fetch(cache.k_pool, k_codes, k_scales);
-            fetch(cache.v_pool, v_codes, v_scales);
-        }
-        uint32_t it = 0;
-        for (int kb = kb_first; kb <= kb_last; ++kb, ++it) {
-            const int s = it % KV_STAGES;
-            const uint32_t free = ((it / KV_STAGES) & 1) ^ 1;
-            unsigned char* tile = kv_s + (size_t)s * L::STAGE_BYTES;
-            if (kb < kb_last) locate(kb + 1);
-            if (!mbar_wait(&k_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 51); break; }
-            make(tile, k_codes, k_scales, k_most);
-            mbar_arrive(&k_full[s]);
-            if (kb < kb_last) fetch(cache.k_pool, k_codes, k_scales);
-            if (!mbar_wait(&v_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 52); break; }
-            make(tile + L::KV_BYTES, v_codes, v_scales, v_most);
-            mbar_arrive(&v_full[s]);
-            if (kb < kb_last) fetch(cache.v_pool, v_codes, v_scales);
-        }
-        const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_most)), v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_most));
-        const bool any = __any_sync(0xffffffffu, strange);
-        if (lane == 0) {
-            atomicMax(&sizes_s[0], k_bits);
-            atomicMax(&sizes_s[1], v_bits);
-            if (any) atomicExch(&sizes_s[2], 1u);
-        }
-    } else if (warp == 4 || warp == 13) {
-        // ------------------------------------------------ MMA issuers, one for each query tile
-        // D f32, A/B f16: S = Q K^T both K-major, N = 64; O = P V with A from TMEM and B MN-major (bit 16), N = HD
-        constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-        const uint32_t one = lane == 0 ? 1u : 0u;
-        const int x = warp == 4 ? 0 : 1, first = first_of(x), last = last_of(x);
-        const uint32_t s_at = tmem_base + L::S_COL + x * 128, o_at = tmem_base + L::O_COL + x * HD;
-        const uint64_t q_desc = desc_sw128(smem_u32(q_s + x * L::Q_BYTES), 16);
-        auto waits = [&](uint64_t* bar, uint32_t parity, int code) {
-            const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-            if (!there && lane == 0) atomicExch(status, code);
-            tc_fence_after();
-            return there;
-        };
-        auto scores = [&](int kb, int half) {                      // (64 rows of a tile are 8,192 bytes)
-            const uint64_t k_desc = desc_sw128(smem_u32(kv_s + (size_t)((kb - kb_first) % KV_STAGES) * L::STAGE_BYTES) + half * 8192, 16);
+            for (int i = 0; i < HD / 8; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                uint32_t v[4];
 #pragma unroll
-            for (int c = 0; c < L::KCH; ++c)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_ss(one, s_at + half * 64, q_desc + c * (BQ * 128 / 16) + 2 * k, k_desc + c * (BKEY * 128 / 16) + 2 * k, idesc_qk, (c | k) ? 1u : 0u);
-            umma_commit(one, &s_full[2 * x + half]);
-        };
-        bool ok = true;
-        uint32_t taken = 0;                                        // key tiles of this query tile whose weights were taken
-        for (int kb = kb_first - 1; kb <= kb_last && ok; ++kb) {   // weights of tile kb, scores of kb + 1
-            const uint32_t it = (uint32_t)(kb - kb_first);
-            const bool weighs = kb >= first && kb <= last, next = kb + 1 <= kb_last, asks = kb + 1 >= first && kb + 1 <= last;
-            if (next) ok = waits(&k_full[(it + 1) % KV_STAGES], ((it + 1) / KV_STAGES) & 1, 54);
-            if (ok && kb + 1 == first) ok = waits(&q_full[x], 0, 53);
-            if (ok && kb >= kb_first) ok = waits(&v_full[it % KV_STAGES], (it / KV_STAGES) & 1, 57);
-#pragma unroll 1
-            for (int half = 0; half < 2 && ok; ++half) {
-                if (weighs) {
-                    ok = waits(&p_ready[2 * x + half], taken & 1, 56);
-                    if (!ok) break;
-                    const uint64_t v_desc = desc_sw128(smem_u32(kv_s + (size_t)(it % KV_STAGES) * L::STAGE_BYTES) + L::KV_BYTES + half * 8192, BKEY * 128);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)                    // 16 keys = 2,048 bytes of V, 8 columns of P
-                        umma_ts(one, o_at, s_at + half * 64 + 8 * k, v_desc + (uint64_t)((2048 * k) >> 4), idesc_pv, (taken | (uint32_t)half | (uint32_t)k) ? 1u : 0u);
-                    umma_commit(one, &o_done[x]);
-                    if (kb == last && half == 1) umma_commit(one, &o_full[x]);
-                }
-                if (asks) scores(kb + 1, half);
+                for (int j = 0; j < 4; ++j) v[j] = half_pair(__uint_as_float(w[j] << 16) * by, __uint_as_float(w[j] & 0xffff0000u) * by);
+                *reinterpret_cast<uint4*>(q_s + x * L::Q_BYTES + tile_byte(r, 8 * i)) = make_uint4(v[0], v[1], v[2], v[3]);
             }
-            if (ok && weighs) ++taken;
-            // (a tile that this query tile does not see is given back as soon as it is there)
-            if (ok && kb >= kb_first) umma_commit(one, &v_empty[it % KV_STAGES]);
-            if (ok && next) umma_commit(one, &k_empty[(it + 1) % KV_STAGES]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&q_full[x]);
         }
-    } else {
-        // ------------------------------------------------ rows
-        const int quarter = warp & 3, x = (warp - 5) >> 2;
-        const int r = quarter * 32 + lane, place = x * BQ + r, pos = pos0 + place;
-        const int first = first_of(x), last = last_of(x);
-        const int lo_row = pos < 0 ? 0 : first_visible_key(pos, window);
-        const int pos_first = pos0 + x * BQ, pos_last = pos0 + min(rows, (x + 1) * BQ) - 1;
-        const int lo_all = pos_last < 0 ? 0 : first_visible_key(pos_last, window);        // the first key that every row of the tile sees
-        const uint32_t s_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::S_COL + x * 128;
-        const uint32_t o_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::O_COL + x * HD;
-        float base_m = 0.f, limit = -INFINITY, l_run = 0.f;        // in log2 units: the base of the weights, what a score may reach
-        if (share == 0 && extras.sink && extras.sink[h] != -INFINITY) {
-            base_m = extras.sink[h] * 1.4426950408889634f;
-            limit = base_m + HEADROOM;
-            l_run = 1.f;
-        }
-        bool ok = first <= last && mbar_wait(&q_full[x], 0, abort_flag);
-        if (!ok && first <= last && lane == 0) atomicExch(status, 58);
-        const float factor = ok ? factor_s[place] : 0.f;
         // (not 0: minus infinity times it is to stay that)
         const float unit_scale = CAPPED ? 1.0f : fmaxf(scale * 1.4426950408889634f * factor, 1e-37f);
         const unsigned long long unit2 = pair_of(unit_scale, unit_scale);
@@ -626,14 +625,12 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             l_run += even + odd;
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
-            mbar_arrive(&p_ready[2 * x + half]);
+            arrive(&p_ready[2 * x + half]);
         }
         if (ok && !mbar_wait(&o_full[x], 0, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 61); }
         tc_fence_after();
         if (shares > 1) {
-            // (every row has waited for its O: no product reads the tiles any more, and what the makers made is all taken; but for the queries
-            // of a share without keys)
-            if (!mbar_wait(&q_full[1], 0, abort_flag) && lane == 0) atomicExch(status, 62);
+            // (every row has waited for its O: no product reads the tiles any more, and what the makers made is all taken)
             asm volatile("bar.sync 1, %0;" ::"n"(2 * BQ) : "memory");
             part_m[place] = limit > -INFINITY ? base_m : -INFINITY;
             part_l[place] = l_run;

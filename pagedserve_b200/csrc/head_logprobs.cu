@@ -190,7 +190,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * ROW_THREADS); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * ROW_THREADS / 32); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -288,9 +288,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                     tmem_ld32(taddr + c, raw);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     const int n = tile * BN + c;
-                    auto release = [&]() {                         // this team's last read of the accumulator is done
+                    // this team's last read of the accumulator is done (one arrival a warp: those of its lanes take turns at the barrier)
+                    auto release = [&]() {
                         tc_fence_before();
-                        arrive_remote(in_first_cta(&acc_empty[buf]));
+                        __syncwarp();
+                        if (lane == 0) arrive_remote(in_first_cta(&acc_empty[buf]));
                     };
                     if (n >= N) {
                         if (c + 32 * TEAMS >= BN) release();
