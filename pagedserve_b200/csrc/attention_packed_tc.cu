@@ -324,7 +324,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    // for a whole warp (arrivals of all its lanes take turns at the barrier: 512 of them a half of a tile cost more than the half's exponentials)
+    // one arrival for a whole warp
     auto arrive = [&](uint64_t* bar) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);

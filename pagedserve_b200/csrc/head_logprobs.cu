@@ -95,6 +95,12 @@ __device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t desc_a, uint
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// one lane of a warp, chosen by the instruction that the compiler knows to choose one: an MMA's operands are then formed once for the warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen != 0;
+}
 __device__ __forceinline__ void commit_pair(uint64_t* bar) {                                  // arrives at this place in both CTAs
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
@@ -229,7 +235,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                 if (!mbar_wait(&empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; atomicExch(status, 43); }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             // D = f32, A = B = bf16, both K-major, N = 256, M = 256 of the pair
             constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((2 * BM) >> 4) << 24);
             uint32_t it = 0, local = 0;
