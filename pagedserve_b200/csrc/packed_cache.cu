@@ -152,9 +152,12 @@ append_kernel(const T* __restrict__ k_src, long long k_stride, const T* __restri
             (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
 }
 
-// A position's words (k or v, head, place in the row) over the threads of a CTA, blockIdx.x = position, blockIdx.y = item; out: pages
+// The words of some positions (k or v, head, place in the row) over the threads of a CTA, blockIdx.y = item. A word waits for four reads in a row (length,
+// row, page, the word): in bfloat16 four positions share the wait (64 requests of 1,000, 12 heads of 64: 76 us with one, 55 with two, 45 with four; its floor
+// is 21), in float32, whose stores take longer than it, one has more CTAs under way (5 of 1,023, 25 heads of 64: 14.0, 15.3, 16.6; floor 8). out: pages
 // [n_items * span / out_page, 2, kv heads, out_page, head_dim], item i's position p in page i * span / out_page + p / out_page. Positions from kv_len on
 // are left as they are; those without a page, too, or (`fill`) become zeros.
+template <typename T> struct Positions { static constexpr int TOGETHER = sizeof(T) == 2 ? 4 : 1; };
 template <typename T>
 __global__ void __launch_bounds__(256)
 unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
@@ -164,33 +167,45 @@ unpack_kernel(const unsigned char* __restrict__ k_pool, const unsigned char* __r
     k_pool = pdl_fresh(k_pool);
     v_pool = pdl_fresh(v_pool);
     const int groups = groups_of(head_dim), words = groups * 4, per_row = 2 * n_kv_heads * words;
-    const int item = blockIdx.y, p = blockIdx.x;
-    if (p >= kv_len[item]) return;
-    const int page = pages.of(item_row ? item_row[item] : item, p);
-    if (page < 0 && !fill) return;
-    const int page_size = 1 << pages.page_log2, row = p & (page_size - 1), out_size = 1 << out_log2;
-    const long long out_page = (long long)item * (span >> out_log2) + (p >> out_log2);
+    constexpr int TOGETHER = Positions<T>::TOGETHER;
+    const int item = blockIdx.y, first = blockIdx.x * TOGETHER, length = kv_len[item], table_row = item_row ? item_row[item] : item;
+    const int page_size = 1 << pages.page_log2, out_size = 1 << out_log2;
+    if (first >= length) return;
+    int page[TOGETHER];
+#pragma unroll
+    for (int u = 0; u < TOGETHER; ++u) page[u] = first + u < length && first + u < span ? pages.of(table_row, first + u) : -1;
     for (int index = threadIdx.x; index < per_row; index += blockDim.x) {
         const int both = index / words, place = index - both * words, plane = both >= n_kv_heads ? 1 : 0, head = both - plane * n_kv_heads;
-        const int part = place / groups, j = place - part * groups, d = j * GROUP + part * 8;
-        uint32_t word = 0, scale = 0;
-        if (page >= 0) {
-            const unsigned char* slab = (plane ? v_pool : k_pool) + (long long)page * page_stride + (long long)head * slab_bytes(page_size, head_dim);
-            word = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
-            scale = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
+        const int part = place / groups, j = place - part * groups, d = j * GROUP + part * 8, count = head_dim - d;
+        const unsigned char* slabs = (plane ? v_pool : k_pool) + (long long)head * slab_bytes(page_size, head_dim);
+        uint32_t word[TOGETHER], scale[TOGETHER];
+#pragma unroll
+        for (int u = 0; u < TOGETHER; ++u) {
+            word[u] = scale[u] = 0u;
+            if (page[u] >= 0) {
+                const int row = first + u & (page_size - 1);
+                const unsigned char* slab = slabs + (long long)page[u] * page_stride;
+                word[u] = reinterpret_cast<const uint32_t*>(slab)[row * words + place];
+                scale[u] = reinterpret_cast<const uint32_t*>(slab + page_size * groups * 16)[row * groups + j];
+            }
         }
-        const float step = step_of(scale), low = low_of(scale);
-        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word >> code_shift(i)) & 15u), step, low);
-        T* to = out + (((out_page * 2 + plane) * n_kv_heads + head) * out_size + (p & (out_size - 1))) * head_dim + d;
-        const int count = head_dim - d;
-        if (count >= 8 && aligned) {
-            Eight<T>::store(to, x);
-        } else {
+        for (int u = 0; u < TOGETHER; ++u) {
+            const int p = first + u;
+            if (p >= length || p >= span || (page[u] < 0 && !fill)) continue;
+            const float step = step_of(scale[u]), low = low_of(scale[u]);
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < count) to[i] = from_float<T>(x[i]);
+            for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word[u] >> code_shift(i)) & 15u), step, low);
+            const long long out_page = (long long)item * (span >> out_log2) + (p >> out_log2);
+            T* to = out + (((out_page * 2 + plane) * n_kv_heads + head) * out_size + (p & (out_size - 1))) * head_dim + d;
+            if (count >= 8 && aligned) {
+                Eight<T>::store(to, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < count) to[i] = from_float<T>(x[i]);
+            }
         }
     }
 }
@@ -213,10 +228,11 @@ template <typename T>
 int unpack(const void* k_pool, const void* v_pool, long long page_stride, const int* kv_len, const int* item_row, const Pages& pages, int n_items,
            int span, void* out, int out_page, int n_kv_heads, int head_dim, int fill, cudaStream_t s) {
     const long long words = (long long)2 * n_kv_heads * groups_of(head_dim) * 4;
-    const int threads = words >= 256 ? 256 : (int)((words + 31) / 32 * 32);
     if (words > 0x7fffffff) return PS_ERR_UNSUPPORTED;
+    const long long rounds = (words + 255) / 256;
+    const int threads = (int)(((words + rounds - 1) / rounds + 31) / 32 * 32);         // (as many in the last round as in the others)
     const int aligned = !((uintptr_t)out & 15) && head_dim % 8 == 0;
-    return launch_pdl(unpack_kernel<T>, dim3(span, n_items), dim3(threads), 0, s, (const unsigned char*)k_pool,
+    return launch_pdl(unpack_kernel<T>, dim3((span + Positions<T>::TOGETHER - 1) / Positions<T>::TOGETHER, n_items), dim3(threads), 0, s, (const unsigned char*)k_pool,
                       (const unsigned char*)v_pool, page_stride, kv_len, item_row, pages, span, (T*)out, log2_of(out_page), n_kv_heads, head_dim,
                       aligned, fill);
 }
