@@ -11,6 +11,9 @@
 // A CTA has a token, a head and a share of its keys: tiles of 32 keys aligned to absolute positions, one tile after another for each
 // warp.  For the scores a lane has a key, for the values the numbers `lane` of every group.  The shares of a token and head are a
 // thread-block cluster and merge through shared memory, in the order of the shares.
+//
+// What bounds it: instructions, a multiply-add, a rotation and a mask for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
+// heads of 64, capped scores, a sink: 10.7 us for 3.2 MB; 8 CTAs a head leave each warp two tiles).
 #include "packed.cuh"
 
 namespace ps {

@@ -3,9 +3,8 @@
 //
 // product     pairs of CTAs on tiles of 256 rows x 256 tokens as in gemm_tc.cu (tcgen05 cta_group::2, TMA, two accumulators in TMEM). A pair keeps
 //             to its 256 rows and walks a strip of the vocabulary, so that the sums of a row stay in the registers of its four threads (each takes
-//             every fourth 32 tokens of a tile); a strip leaves m, S and W of its part of a row.  A tile of 768 deep is 8,600 clocks of
-//             the tensor pipe; a warp reads 32 tokens of its rows in about 2,300, most of them waits for results, so that with two threads a
-//             row the reading was as long as the product.
+//             every fourth 32 tokens of a tile); a strip leaves m, S and W of its part of a row.  A warp reads 32 tokens of its rows in about
+//             2,300 clocks, most of them waits for results, so that with two threads a row the reading was longer than the product.
 // sample      for the most likely tokens, the logits of every s-th token (about 2,048 of them) are formed first, by the ordinary product: the `top`-th
 //             largest of them is a bound that the row's `top` largest reach, less 2^-16 of itself, since another product may add in another order.
 //             The product sends what lies beyond it (about 25 * top of 50,257) to a list of its row: a number larger than the bound, or equal to it
@@ -14,6 +13,10 @@
 //             wait: 326 us of 445; one for each row that had eight, 157 of 266 us with 20 alternatives).
 // join        a CTA a row adds the strips' sums up, ranks the list, and writes the results.  A row whose list did not hold all (an order of tokens that
 //             fools the sample), or fewer than `top`, has its logits formed again there, token by token.
+//
+// What bounds it, 2,047 rows of 768 on 50,257 tokens (158 GFLOP, 96 us at a cuBLAS product's measured rate): without alternatives the tensor pipe, 94 us
+// (112 with the MMAs issued behind `lane == 0` instead of elect.sync); with 5 of them 157, of which the sample's product and ranking are about 25, the join 13,
+// and numbers on their way to the lists 10; with 20 183. Up to about 256 rows (42 us) the table's 77 MB and four kernels one behind another.
 #include <cuda.h>
 
 #include "logprobs.cuh"

@@ -14,6 +14,9 @@
 // holds (rising logits), the four chunks are read once more, each behind a bound of its own, which adds at most a chunk's numbers.
 //
 // A row is one CTA, or the CTAs of a cluster that share its columns out (few rows).
+//
+// What bounds it, rows of 50,257: without alternatives the bytes (2,047 rows, 412 MB: 74 us, 5.6 TB/s); with them the list, its looks and rankings (5
+// alternatives 121 us, 20 131, 32 145); 8 rows 10.3 us, one trip through a share's eighth of a row and the shares' join.
 #include "logprobs.cuh"
 
 namespace ps {
