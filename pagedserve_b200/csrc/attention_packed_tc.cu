@@ -366,12 +366,19 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         float k_most = 0.f, v_most = 0.f;
         long long page_at = -1;                                    // of the key whose numbers are asked for (below 0: not needed, or no page)
         int page_row = 0;
+        // A key's entry of the block table is asked for a tile before its codes, and not looked at until then: a comparison would wait for it.
+        const int* table = cache.pages.block_table + (size_t)table_row * cache.pages.bt_stride;
+        auto needed = [&](int kb) { return kb * BKEY + r >= lo && kb * BKEY + r <= hi; };
+        auto entry_of = [&](int kb) {
+            const int at = (kb * BKEY + r) >> cache.pages.page_log2;
+            return needed(kb) && at < cache.pages.bt_stride ? table[at] : -1;
+        };
+        int entry = entry_of(kb_first);
         auto locate = [&](int kb) {
-            const int key = kb * BKEY + r;
-            const bool needed = key >= lo && key <= hi;
-            const int page = needed ? cache.pages.of(table_row, key) : -1;
-            strange |= needed && page < 0;
-            page_row = key & (page_size - 1);
+            const int page = entry < cache.pages.n_pages ? entry : -1;
+            entry = entry_of(kb + 1);
+            strange |= needed(kb) && page < 0;
+            page_row = (kb * BKEY + r) & (page_size - 1);
             page_at = page < 0 ? -1 : (long long)page * cache.page_stride + head_at;
         };
         auto fetch = [&](const unsigned char* pool, uint4 (&codes)[GROUPS_MOST], uint32_t (&scales)[GROUPS_MOST]) {
