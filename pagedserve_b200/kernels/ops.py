@@ -2314,21 +2314,22 @@ class Ops:
         """Checks what the log probabilities' entry points share; the tensors that take the results."""
         if max(rows, vocabulary) > MOST_COUNT:
             raise KernelError(f"{what}: rows and vocabularies of up to {MOST_COUNT}")
-        _require(targets, "targets", torch.int32)
-        if targets.ndim != 1 or targets.numel() != rows or not targets.is_contiguous() or targets.device != device:
+        if not (targets.dtype is torch.int32 and targets.ndim == 1 and targets.shape[0] == rows and targets.is_contiguous()
+                and targets.get_device() == device and device >= 0 and device == _device_number()):
+            _require(targets, "targets", torch.int32)
+            self._on_current_device(what, targets)
             raise KernelError(f"{what}: one int32 token per row, on the device of the rows")
         if not (0 <= top <= min(vocabulary, MOST_ALTERNATIVES)):
             raise KernelError(f"{what}: top is 0 to {MOST_ALTERNATIVES}, and at most the vocabulary")
-        self._on_current_device(what, targets)
         if results is not None:
             for name, shape, dtype in (("logprob", (rows,), torch.float32), ("entropy", (rows,), torch.float32),
                                        ("top_logprobs", (rows, top), torch.float32), ("top_ids", (rows, top), torch.int32)):
                 tensor = getattr(results, name)
-                if tensor.shape != shape or tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.device != device:
+                if tensor.shape != shape or tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.get_device() != device:
                     raise KernelError(f"{what}: results.{name} must be contiguous {shape} in {dtype}, on the device of the rows")
             return results
-        numbers = torch.empty((2 + top, rows), dtype=torch.float32, device=device)
-        return TokenLogprobs(numbers[0], numbers[1], numbers[2:].view(rows, top), targets.new_empty((rows, top)))
+        logprob, entropy = targets.new_empty((2, rows), dtype=torch.float32).unbind()        # (a tensor operation costs the host 1 to 2 us)
+        return TokenLogprobs(logprob, entropy, targets.new_empty((rows, top), dtype=torch.float32), targets.new_empty((rows, top)))
 
     def token_logprobs(self, logits, targets, top=0, status=None, results=None):
         """:class:`TokenLogprobs` of float32 ``logits`` [rows, vocabulary] and one token a row (int32): its log probability under the row's softmax,
@@ -2338,17 +2339,18 @@ class Ops:
         contiguous and of these shapes."""
         what = "token_logprobs"
         _require(logits, "logits", torch.float32)
-        if logits.ndim != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
+        shape = logits.shape
+        if len(shape) != 2 or shape[1] == 0 or logits.stride(1) != 1:
             raise KernelError(f"{what}: logits must be rows of a vocabulary")
-        rows, V = logits.shape
-        results = self._logprob_results(what, rows, V, targets, top, logits.device, results)
+        rows, V = shape
+        results = self._logprob_results(what, rows, V, targets, top, logits.get_device(), results)
         if rows == 0:
             return results
         ld = logits.stride(0) if rows > 1 else V
         if ld < V:
             raise KernelError(f"{what}: the rows of logits overlap")
         if status is None:
-            status = self.status_flag(logits.device)
+            status = self.status if self.status is not None else self.status_flag(logits.device)
         self.launches += 1
         _check(self._packed_library().ps_token_logprobs(_ptr(logits), ld, rows, V, _ptr(targets), top, _ptr(results.logprob), _ptr(results.entropy),
                                            _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), what)
@@ -2400,7 +2402,7 @@ class Ops:
         if x.stride(1) != 1 or table.stride(1) != 1 or x.device != table.device:
             raise KernelError(f"{what}: x and table must be rows on one device")
         rows, V = x.shape[0], table.shape[0]
-        results = self._logprob_results(what, rows, V, targets, top, x.device)
+        results = self._logprob_results(what, rows, V, targets, top, x.get_device())
         if status is None:
             status = self.status_flag(x.device)
         if self.fused_head_ok(x, table):

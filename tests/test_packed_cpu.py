@@ -88,7 +88,7 @@ def test_counts_beyond_32_bits_are_refused():
     ops, targets = Ops(torch.float32), torch.zeros(1, dtype=torch.int32)
     for rows, vocabulary in ((2 ** 31 - 1, 10), (1, 2 ** 31 - 1), (1, 2 ** 32 + 5)):
         with pytest.raises(KernelError, match="of up to"):
-            ops._logprob_results("token_logprobs", rows, vocabulary, targets, 0, targets.device)
+            ops._logprob_results("token_logprobs", rows, vocabulary, targets, 0, targets.get_device())
 
 
 def test_declared_arguments_are_the_sources():
