@@ -16,7 +16,7 @@
 //
 // What bounds it, 2,047 rows of 768 on 50,257 tokens (158 GFLOP, 96 us at a cuBLAS product's measured rate): without alternatives the tensor pipe, 94 us
 // (112 with the MMAs issued behind `lane == 0` instead of elect.sync); with 5 of them 157, of which the sample's product and ranking are about 25, the join 13,
-// and numbers on their way to the lists 10; with 20 183. Up to about 256 rows (42 us) the table's 77 MB and four kernels one behind another.
+// and numbers on their way to the lists 10; with 20 183. Up to about 256 rows (42 us; without alternatives 21) the table's 77 MB and four kernels one behind another.
 #include <cuda.h>
 
 #include "logprobs.cuh"

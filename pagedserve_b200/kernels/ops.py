@@ -2356,12 +2356,18 @@ class Ops:
                                            _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), what)
         return results
 
-    FUSED_HEAD_ROWS, FUSED_HEAD_VOCABULARY, FUSED_HEAD_MOST, SAMPLED = 96, 8192, 4096, 2048
+    FUSED_HEAD_VOCABULARY, FUSED_HEAD_MOST, SAMPLED = 8192, 4096, 2048
 
-    def fused_head_ok(self, x, table):
-        """Whether the log probabilities of these rows are read inside the head's product: many rows of a large vocabulary in bfloat16."""
-        return (self.dtype == torch.bfloat16 and x.shape[0] >= self.FUSED_HEAD_ROWS and table.shape[0] >= self.FUSED_HEAD_VOCABULARY
-                and self.tc_ok(x, table))
+    def fused_head_ok(self, x, table, top=0):
+        """Whether the log probabilities of these rows are read inside the head's product: bfloat16, a large vocabulary, and so many rows that the
+        logits' way to memory and back takes longer than what stands around that product.
+
+        Inside / formed first, us: without alternatives 8 rows of 768 on 50,257 tokens 21.8 / 20.6, 16 22.9 / 26.1, 64 23.0 / 44.4; of 1,024 on 32,000 at 16
+        rows 21.2 / 24.5; of 768 on 9,000 11.4 / 12.2. With 5, whose sample and list are four kernels more: on 50,257 at 40 rows 36.3 / 34.5, 48 35.9 / 46.2,
+        96 39.1 / 43.7; on 32,000 at 33 rows 32.1 / 26.4, 64 32.3 / 42.0, 96 36.9 / 33.5, 128 36.7 / 37.1; on 9,000 at 128 27.4 / 27.0."""
+        rows, V = x.shape[0], table.shape[0]
+        least = 16 if not top else 48 if V > 40000 else 128
+        return self.dtype == torch.bfloat16 and rows >= least and V >= self.FUSED_HEAD_VOCABULARY and self.tc_ok(x, table)
 
     def _fused_head(self, x, table, targets, top, status, results):
         (rows, K), V, device = x.shape, table.shape[0], x.device
@@ -2405,7 +2411,7 @@ class Ops:
         results = self._logprob_results(what, rows, V, targets, top, x.get_device())
         if status is None:
             status = self.status_flag(x.device)
-        if self.fused_head_ok(x, table):
+        if self.fused_head_ok(x, table, top):
             for start in range(0, rows, self.FUSED_HEAD_MOST):
                 part = slice(start, min(rows, start + self.FUSED_HEAD_MOST))
                 self._fused_head(x[part], table, targets[part], top, status, TokenLogprobs(*(result[part] for result in results)))

@@ -130,6 +130,19 @@ def test_heads_that_fool_a_sample(kind, rows):
     check(found, logits, targets, top)
 
 
+@pytest.mark.parametrize("top", [0, 4])
+@pytest.mark.parametrize("rows,width,V", [(15, 64, 8192), (16, 64, 8192), (17, 200, 41000), (47, 96, 40001), (48, 96, 40001), (127, 64, 9001), (128, 72, 9001)])
+def test_rows_around_the_choice_of_a_form(rows, width, V, top):
+    """Read inside the product or from logits: numbers on a grid whose sums are exact, as above."""
+    ops = ops_for(torch.bfloat16)
+    g = torch.Generator(device=DEV).manual_seed(rows + width)
+    x = ((torch.randn(rows, width, generator=g, device=DEV) * 8).round() / 8).clamp(-6, 6).bfloat16()
+    table = ((torch.randn(V, width, generator=g, device=DEV) * 20).round() / 512).clamp(-0.49, 0.49).bfloat16()
+    targets = torch.randint(-1, V, (rows,), generator=g, device=DEV).int()
+    assert ops.fused_head_ok(x, table, top) == (rows >= (16 if not top else 48 if V > 40000 else 128))
+    check(ops.head_logprobs(x, table, targets, top), x.double() @ table.double().t(), targets, top)
+
+
 @pytest.mark.parametrize("rows,width,V", [(96, 768, 20000), (300, 200, 9000), (1500, 1600, 8500)])
 def test_tokens_with_the_same_row_of_the_table(rows, width, V):
     """Equal logits whose sums are rounded: the lower tokens, in order, whichever of them a sample of the vocabulary holds."""
