@@ -20,14 +20,14 @@
 // What bounds it: instructions, not bytes (the same time with one page that every token shares). A tile of 16 keys is about 600 instructions a warp at
 // 128 numbers a head and 8 queries, half of them masks, shifts and sums on the ALU pipe, which issues every other clock (44 - 51 % busy; a warp's own chain
 // of scores, weights and products leaves the rest idle); its 32 mma.sync are not felt. 64 tokens of 4,099 keys, 32 heads on 8 of 128: 102 us, 2.3 TB/s;
-// 64 x 1,024, 12 heads of 64: 28 us; one token of 32,768: 36 us, 12 CTAs a cluster share of 8 on 148 SMs. A page's number is asked for a tile before it
-// is used and not compared until then, or its latency stands in the loop (110 and 46 us).
+// 64 x 1,024, 12 heads of 64: 28 us; one token of 32,768: 26 us, 12 heads by 8 shares of 8 warps on 148 SMs. A page's number is asked for a tile before it
+// is used and not compared until then, or its latency stands in the loop (110 us; one token 46, so 36 with 4 warps).
 #include "packed.cuh"
 
 namespace ps {
 namespace packed {
 
-constexpr int M_WARPS = 4, M_KEYS = 16;
+constexpr int M_KEYS = 16;
 constexpr float HEADROOM = 8.f;                            // log2 of how far a weight may be beyond 1 before its base moves
 constexpr int LEAST_EXPONENT = 27, MOST_EXPONENT = 253;    // biased: steps below 2^-100 count as that, those from 2^126 on (up to 4 of it)
 
@@ -90,20 +90,20 @@ __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)
 }
 
 // a tile in the ring: codes of 16 keys, codes of 16 values, their scales
-template <int NG>
+template <int NG, int M_WARPS>
 struct Ring {
     static constexpr int CODES = M_KEYS * NG * 16, SCALES = M_KEYS * NG * 4, TILE_BYTES = 2 * (CODES + SCALES);
     static constexpr int STAGES = NG <= 2 ? 4 : 3;
     static constexpr int BYTES = M_WARPS * STAGES * TILE_BYTES;
 };
 
-template <int NG, int NQ>
-__global__ void __launch_bounds__(M_WARPS * 32, (NG * NQ <= 4 ? 4 : 2))
+template <int NG, int NQ, int M_WARPS>
+__global__ void __launch_bounds__(M_WARPS * 32, (NG * NQ <= 4 ? 4 : 2) * 4 / M_WARPS)
 tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __restrict__ out, long long out_stride, int wide,
                   const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
                   const int* __restrict__ token_row, const int* __restrict__ positions, Pages pages, int n_heads, int n_kv_heads, int head_dim,
                   int window, float scale, float softcap, const float* __restrict__ sink, int aligned) {
-    using R = Ring<NG>;
+    using R = Ring<NG, M_WARPS>;
     constexpr int COLUMNS = 8 * NQ, NUMBERS = NG * GROUP;
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ float base_s[M_WARPS][COLUMNS], sum_s[M_WARPS][COLUMNS], share_base[COLUMNS], share_sum[COLUMNS];
@@ -499,13 +499,13 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     if (shares > 1) cluster_sync_all();                          // the shares stay until they were read
 }
 
-template <int NG, int NQ>
+template <int NG, int NQ, int M_WARPS>
 int launch_mma(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
                long long page_stride, const int* token_row, const int* positions, const Pages& pages, int tokens, int n_heads, int n_kv_heads,
                int head_dim, int window, float scale, float softcap, const float* sink, int shares, cudaStream_t s) {
     constexpr int COLUMNS = 8 * NQ, MERGE = M_WARPS * COLUMNS * NG * GROUP * 4;
-    constexpr size_t SMEM = Ring<NG>::BYTES > MERGE ? Ring<NG>::BYTES : MERGE;
-    auto kernel = tokens_mma_kernel<NG, NQ>;
+    constexpr size_t SMEM = Ring<NG, M_WARPS>::BYTES > MERGE ? Ring<NG, M_WARPS>::BYTES : MERGE;
+    auto kernel = tokens_mma_kernel<NG, NQ, M_WARPS>;
     static size_t raised[MAX_DEVICES] = {0};
     if (!ensure_dynamic_smem((const void*)kernel, SMEM, raised)) return PS_ERR_LAUNCH;
     const int ratio = n_heads / n_kv_heads, blocks = (ratio + COLUMNS - 1) / COLUMNS;
@@ -522,23 +522,25 @@ int launch_mma(const void* q, long long q_stride, void* out, long long out_strid
 PS_EXPORT int ps_packed_tokens_mma(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool,
                                    const void* v_pool, int n_pages, long long page_stride, const int* token_row, const int* positions,
                                    const int* block_table, int bt_stride, int tokens, int n_heads, int n_kv_heads, int head_dim, int page_size,
-                                   int window, float scale, float softcap, const float* sink, int shares, void* stream) {
+                                   int window, float scale, float softcap, const float* sink, int shares, int warps, void* stream) {
     using namespace ps::packed;
     if (tokens <= 0) return PS_OK;
     if (!q || !out || !k_pool || !v_pool || !token_row || !positions || !block_table) return PS_ERR_BAD_ARGUMENT;
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return PS_ERR_BAD_ARGUMENT;
     if (!sizes_ok(n_kv_heads, head_dim, page_size) || head_dim > 128 || n_heads > 65535) return PS_ERR_UNSUPPORTED;
     if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
-    if (shares != 1 && shares != 2 && shares != 4 && shares != 8) return PS_ERR_BAD_ARGUMENT;
+    if ((shares != 1 && shares != 2 && shares != 4 && shares != 8) || (warps != 4 && warps != 8)) return PS_ERR_BAD_ARGUMENT;
     const Pages pages = {block_table, bt_stride, n_pages, log2_of(page_size)};
     const bool two = n_heads / n_kv_heads > 8;
-#define PS_PACKED_MMA(NG, NQ)                                                                                                                \
-    return launch_mma<NG, NQ>(q, q_stride, out, out_stride, wide, k_pool, v_pool, page_stride, token_row, positions, pages, tokens, n_heads, \
-                              n_kv_heads, head_dim, window, scale, softcap, sink, shares, (cudaStream_t)stream)
-#define PS_PACKED_MMA_GROUPS(NG)          \
-    case NG:                              \
-        if (two) PS_PACKED_MMA(NG, 2);    \
-        PS_PACKED_MMA(NG, 1)
+#define PS_PACKED_MMA(NG, NQ, W)                                                                                                             \
+    return launch_mma<NG, NQ, W>(q, q_stride, out, out_stride, wide, k_pool, v_pool, page_stride, token_row, positions, pages, tokens,       \
+                                 n_heads, n_kv_heads, head_dim, window, scale, softcap, sink, shares, (cudaStream_t)stream)
+#define PS_PACKED_MMA_GROUPS(NG)                         \
+    case NG:                                             \
+        if (two && warps == 8) PS_PACKED_MMA(NG, 2, 8);  \
+        if (two) PS_PACKED_MMA(NG, 2, 4);                \
+        if (warps == 8) PS_PACKED_MMA(NG, 1, 8);         \
+        PS_PACKED_MMA(NG, 1, 4)
     switch (groups_of(head_dim)) {
         PS_PACKED_MMA_GROUPS(1);
         PS_PACKED_MMA_GROUPS(2);

@@ -138,7 +138,7 @@ _SIGNATURES = {
         "ps_kv_append_packed": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P],
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
-        "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P],
+        "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P, _P],
         "ps_head_logprobs_strips": [_I, _I],
         "ps_head_logprobs": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P],
@@ -1300,11 +1300,11 @@ class Ops:
         return rows
 
     def packed_attention_tokens(self, q, out, k_pool, v_pool, page_stride, token_row, positions, block_table, n_heads, n_kv_heads, head_dim,
-                                page_size, window, scale, max_kv_len, softcap=None, sink=None, shares=0):
+                                page_size, window, scale, max_kv_len, softcap=None, sink=None, shares=0, warps=0):
         """Attention of single tokens over a packed cache: token t, at ``positions[t]``, reads the pages of row ``token_row[t]`` of
         ``block_table``.  ``max_kv_len`` bounds every token's context (it fixes the grid, so a CUDA graph passes the longest).  ``out`` may be float32
-        in bfloat16.  A token at a position below 0 sees nothing: its row becomes zero.  ``shares``: CTAs for the keys of a token, 1, 2, 4 or 8 (0: by the
-        counts).  Otherwise as :meth:`paged_attention_decode`."""
+        in bfloat16.  A token at a position below 0 sees nothing: its row becomes zero.  ``shares``: CTAs for the keys of a token, 1, 2, 4 or 8, ``warps``
+        (bfloat16, heads of up to 128): those of a CTA, 4 or 8 (0: by the counts).  Otherwise as :meth:`paged_attention_decode`."""
         what = "packed_attention_tokens"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
@@ -1324,10 +1324,16 @@ class Ops:
                 while shares < 8 and (ctas * shares * 2 <= 592 and shares * 2 <= keys // 128
                                       or ctas * shares * 2 <= 1184 and shares * 2 <= keys // 1024):
                     shares *= 2
+            if not warps:
+                # Twice the warps a CTA where a cluster cannot be larger and each warp has 8 tiles of keys or more, and where they are resident as well as
+                # half of them twice (us with 4 / 8: 1 x 32,768, 12 heads of 64, 35.8 / 26.5; 1 x 8,192 12.7 / 10.6; 4 x 16,000, 32 heads on 8 of 128, 42.3 /
+                # 36.8; 16 x 2,048, 16 on 2 of 64, 7.9 / 8.7; 16 x 4,000, 32 on 2 of 128, two column blocks a warp, 18.3 / 33.6).
+                ratio = n_heads // n_kv_heads
+                warps = 8 if shares == 8 and keys >= 4096 and (ratio <= 8 or T * n_kv_heads * -(-ratio // 16) * 8 <= 148) else 4
             _check(self._packed_library().ps_packed_tokens_mma(
                 _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
                 page_stride, _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim,
-                page_size, window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, _stream()), what)
+                page_size, window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, warps, _stream()), what)
             return out
         if not shares:
             shares, most = 1, keys // 128

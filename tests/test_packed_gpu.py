@@ -203,6 +203,26 @@ def test_long_contexts_and_many_tokens(dtype, tokens, length):
         assert ((out.cpu().double().view(tokens, heads, dim) - want).abs() <= limit).all()
 
 
+@pytest.mark.parametrize("shares,warps", [(1, 4), (1, 8), (2, 8), (4, 8), (8, 4), (8, 8)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 32), (6, 2, 64), (3, 3, 96), (8, 1, 128), (20, 2, 128)])
+def test_shares_and_warps_of_single_tokens(shares, warps, heads, kv_heads, dim):
+    """Contexts of fewer keys than warps, of one, of none."""
+    ops, page, lengths = ops_for(BF16), 16, [1200, 17, 1, 333]
+    case = PackedCase(lengths, kv_heads, dim, page, BF16, seed=dim)
+    _, planes = on_device(case)
+    q = torch.randn(5, heads * dim, generator=torch.Generator().manual_seed(1)).bfloat16()
+    out = torch.full((5, heads * dim), 7.0, device=DEV)
+    at = [1199, 16, 0, 332, -1]
+    ops.packed_attention_tokens(q.to(DEV), out, *planes, ints([0, 1, 2, 3, 0]), ints(at), case.table.to(DEV), heads, kv_heads, dim, page, None, 0.125, 1200,
+                                shares=shares, warps=warps)
+    assert (out[4] == 0).all()
+    held_k, held_v = case.held()
+    for i in range(4):
+        want, weighted, sizes = attention(q[i:i + 1].double().view(1, heads, dim), case.context(i, held_k), case.context(i, held_v), torch.tensor([at[i]]), 0.125)
+        limit = bound_of(want, weighted, sizes, 0.125, F32, 2.0 ** -11, dim)
+        assert ((out[i:i + 1].cpu().double().view(1, heads, dim) - want).abs() <= limit).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("k_scale,v_scale,q_scale", [(1e4, 1e6, 1e-4), (1e-6, 1e-9, 1e3), (1.0, 3e30, 1.0), (1.0, 1e-30, 1.0), (3e5, 1.0, 2e5), (0.0, 0.0, 1.0)])
 def test_sizes_of_numbers(dtype, k_scale, v_scale, q_scale):
