@@ -4,15 +4,15 @@
 // A key reads as low_j + step_j c in group j, so that
 //   q . k = sum over j of step_j (q_j . c_j) + low_j sum(q_j)           (q_j, c_j: the numbers and codes of group j)
 // and the weighted values are sum over keys of (p step_j) c + sum over keys of p low_j: a code is met by one multiply-add, the group's two numbers once a key.
-// A code is put into the mantissa of 16.0 (a rotation and a mask: 16 + c exactly) and moved to the middle of its range, c - 8, with low_j + 8 step_j
-// in place of low_j: sums of 16 + c, eight times as large, cost the float32 results a digit (5 tokens, 512 keys, heads of 64: 2.4e-6 off, so
+// A code is put into the mantissa of a power of two (a value's into that of 16, by a rotation and a mask; two of a key's into those of 2^23, by a byte
+// permutation each, for packed additions and multiply-adds) and moved to the middle of its range, c - 8, with low_j + 8 step_j in place of low_j: sums of 16 + c, eight times as large, cost the float32 results a digit (5 tokens, 512 keys, heads of 64: 2.4e-6 off, so
 // 3e-7).  Scores, weights, sums: float32.
 //
 // A CTA has a token, a head and a share of its keys: tiles of 32 keys aligned to absolute positions, one tile after another for each
 // warp.  For the scores a lane has a key, for the values the numbers `lane` of every group.  The shares of a token and head are a
 // thread-block cluster and merge through shared memory, in the order of the shares.
 //
-// What bounds it: instructions, a multiply-add, a rotation and a mask for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
+// What bounds it: instructions, two to four for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
 // heads of 64, capped scores, a sink: 10.7 us for 3.2 MB; 8 CTAs a head leave each warp two tiles).
 #include "packed.cuh"
 
@@ -25,7 +25,12 @@ constexpr int WARPS = 4, TILE = 32;
 __device__ __forceinline__ float centred(uint32_t word, int rotation) {
     return __uint_as_float((__funnelshift_l(word, word, rotation) & 0x00780000u) | 0x41800000u) - 24.f;
 }
-__host__ __device__ __forceinline__ int rotation_of(int i) { return (19 - code_shift(i)) & 31; }
+// bytes B and B + 2 of a word of codes, one a byte, as codes - 8: a byte put into the mantissa of 2^23, less 2^23 + 8
+template <int B>
+__device__ __forceinline__ unsigned long long centred_pair(uint32_t codes) {
+    const float x = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7540 + B)), y = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7542 + B));
+    return pair_add(pair_of(x, y), pair_of(-8388616.f, -8388616.f));
+}
 
 template <typename T, int NG>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -81,30 +86,32 @@ tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ ou
         if (page >= 0) {
             const uint4* codes = reinterpret_cast<const uint4*>(k_pool + at) + row * NG;
             const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pool + at + words_at) + row * NG;
-            float dot[NG];
+            unsigned long long dot[NG];                            // sums over even and over odd numbers
 #pragma unroll
-            for (int j = 0; j < NG; ++j) dot[j] = 0.f;
+            for (int j = 0; j < NG; ++j) dot[j] = 0ull;
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
                 const uint4 raw = codes[u];
                 const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    constexpr int LAST = NG;
                     const int place = u * 4 + w;
-                    const float4 a = *reinterpret_cast<const float4*>(q_s + place * 8), b = *reinterpret_cast<const float4*>(q_s + place * 8 + 4);
-                    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                    float sum = dot[place % LAST];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum = fmaf(centred(word[w], rotation_of(i)), x[i], sum);
-                    dot[place % LAST] = sum;
+                    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(q_s + place * 8), b = *reinterpret_cast<const ulonglong2*>(q_s + place * 8 + 4);
+                    const uint32_t low = word[w] & 0x0f0f0f0fu, high = word[w] >> 4 & 0x0f0f0f0fu;       // numbers 0, 4, 1, 5 and 2, 6, 3, 7
+                    unsigned long long sum = dot[place % NG];
+                    sum = pair_fma(centred_pair<0>(low), a.x, sum);
+                    sum = pair_fma(centred_pair<0>(high), a.y, sum);
+                    sum = pair_fma(centred_pair<1>(low), b.x, sum);
+                    dot[place % NG] = pair_fma(centred_pair<1>(high), b.y, sum);
                 }
             }
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 const uint32_t two = words[j];
-                sum = fmaf(step_of(two), dot[j], fmaf(fmaf(8.f, step_of(two), low_of(two)), q_sum[j], sum));
+                float even, odd;
+                pair_split(dot[j], even, odd);
+                sum = fmaf(step_of(two), even + odd, fmaf(fmaf(8.f, step_of(two), low_of(two)), q_sum[j], sum));
             }
             s = softcap > 0.f ? softcap * 1.4426950408889634f * tanhf(sum * (scale / softcap)) : sum * scale_log2;
         }
