@@ -13,7 +13,8 @@
 // thread-block cluster and merge through shared memory, in the order of the shares.
 //
 // What bounds it: instructions, two to four for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
-// heads of 64, capped scores, a sink: 10.7 us for 3.2 MB; 8 CTAs a head leave each warp two tiles).
+// heads of 64, capped scores, a sink: 8.6 us for 3.2 MB; 64 tokens of 1,024 keys, 12 heads of 64, 34.6), and for few tokens the chain of page, keys, weights and values of a tile: the values of
+// 16 keys (2 groups a head) are on their way while the scores are formed (one token of 32,768 keys 61 us; with four at a time, asked for when they are due, 101).
 #include "packed.cuh"
 
 namespace ps {
@@ -38,7 +39,7 @@ tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ ou
               const unsigned char* __restrict__ k_pool, const unsigned char* __restrict__ v_pool, long long page_stride,
               const int* __restrict__ token_row, const int* __restrict__ positions, Pages pages, int n_heads, int n_kv_heads, int head_dim,
               int window, float scale, float softcap, const float* __restrict__ sink) {
-    constexpr int NUMBERS = NG * GROUP;
+    constexpr int NUMBERS = NG * GROUP, BATCH = NG <= 2 ? 16 : NG <= 4 ? 8 : 4;      // keys whose values are under way together
     __shared__ __align__(16) float q_s[NUMBERS];           // in the order of the cache's words
     __shared__ float sum_s[NG];                             // of each group's queries
     __shared__ float weight_s[WARPS][TILE][NG];
@@ -76,12 +77,33 @@ tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ ou
 #pragma unroll
     for (int j = 0; j < NG; ++j) acc[j] = lows[j] = 0.f;
     const int my_rotation = (19 - code_shift(lane & 7)) & 31, my_part = lane >> 3;
-    for (int tile = lo / TILE + share * WARPS + warp; tile * TILE <= last; tile += shares * WARPS) {
+    // (a key's entry of the block table is asked for a tile before, and not looked at until then: a comparison would wait for it)
+    const int* table = pages.block_table + (size_t)table_row * pages.bt_stride;
+    auto entry_of = [&](int tile) {
         const int key = tile * TILE + lane;
-        const bool seen = key >= lo && key <= last;
-        const int page = seen ? pages.of(table_row, key) : -1;
+        return key >= lo && key <= last ? table[key >> pages.page_log2] : -1;
+    };
+    const int first_tile = lo / TILE + share * WARPS + warp;
+    int entry = entry_of(first_tile);
+    for (int tile = first_tile; tile * TILE <= last; tile += shares * WARPS) {
+        const int key = tile * TILE + lane, page = entry < pages.n_pages ? entry : -1;
+        entry = entry_of(tile + shares * WARPS);
         const long long at = page < 0 ? -1 : (long long)page * page_stride + head_at;
         const int row = key & (page_size - 1);
+        // the values' words of the first keys, which the scores do not wait for
+        __syncwarp();                                          // (the last tile's rows and weights are done with)
+        row_s[warp][lane] = page < 0 ? -1 : at + row * NG * 16;
+        __syncwarp();
+        uint32_t value[BATCH][NG];
+        auto load_values = [&](int k0) {
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const long long from = row_s[warp][k0 + k];
+#pragma unroll
+                for (int j = 0; j < NG; ++j) value[k][j] = from < 0 ? 0u : reinterpret_cast<const uint32_t*>(v_pool + from)[my_part * NG + j];
+            }
+        };
+        load_values(0);
         float s = -INFINITY;
         if (page >= 0) {
             const uint4* codes = reinterpret_cast<const uint4*>(k_pool + at) + row * NG;
@@ -119,7 +141,6 @@ tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ ou
         m = m_new;
         const float weight = page >= 0 ? exp2f(s - base) : 0.f;
         l = fmaf(l, shrink, weight);
-        row_s[warp][lane] = page < 0 ? -1 : at + row * NG * 16;
         if (page >= 0) {
             const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + at + words_at) + row * NG;
 #pragma unroll
@@ -131,20 +152,27 @@ tokens_kernel(const T* __restrict__ q, long long q_stride, void* __restrict__ ou
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NG; ++j) lows[j] *= shrink;
+            for (int j = 0; j < NG; ++j) {
+                weight_s[warp][lane][j] = 0.f;
+                lows[j] *= shrink;
+            }
         }
 #pragma unroll
         for (int j = 0; j < NG; ++j) acc[j] *= shrink;
         __syncwarp();
-#pragma unroll 4
-        for (int k = 0; k < TILE; ++k) {
-            const long long from = row_s[warp][k];
-            if (from < 0) continue;
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + from) + my_part * NG;
+#pragma unroll 1
+        for (int k0 = 0; k0 < TILE; k0 += BATCH) {
+            float number[BATCH][NG];
 #pragma unroll
-            for (int j = 0; j < NG; ++j) acc[j] = fmaf(centred(words[j], my_rotation), weight_s[warp][k][j], acc[j]);
+            for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                for (int j = 0; j < NG; ++j) number[k][j] = centred(value[k][j], my_rotation);
+            if (k0 + BATCH < TILE) load_values(k0 + BATCH);
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                for (int j = 0; j < NG; ++j) acc[j] = fmaf(number[k][j], weight_s[warp][k0 + k][j], acc[j]);
         }
-        __syncwarp();
     }
     // the warps' states, then the shares'
     l = warp_sum(l);

@@ -1336,8 +1336,10 @@ class Ops:
                 page_size, window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, warps, _stream()), what)
             return out
         if not shares:
-            shares, most = 1, keys // 128
-            while shares < 8 and T * n_heads * shares * 2 <= 2 * 148 * 8 and shares * 2 <= most:
+            # As above, one head a CTA (us at 1, 2, 4, 8 shares: 1 x 129 keys, 12 heads of 64, 5.9, 5.5, 5.4, 6.0; 8 x 1,024 16.7, 11.7, 10.8, 13.1; 16 x 2,048, 16 heads on
+            # 2 of 64, 34.5, 31.5, 28.3, 33.3; 16 x 4,000, 32 on 8 of 128, 148, 125, 127, 154; 64 x 1,024, 12 of 64, 34.4, 34.9, 42.8, 67.4).
+            ctas, shares = T * n_heads, 1
+            while shares < 8 and (ctas * shares * 2 <= 592 and shares * 2 <= keys // 64 or ctas * shares * 2 <= 1184 and shares * 2 <= keys // 512):
                 shares *= 2
         _check(self._packed_library().ps_packed_tokens_simt(
             _ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(out.dtype), _ptr(k_pool), _ptr(v_pool), n_pages, page_stride,
