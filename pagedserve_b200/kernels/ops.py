@@ -137,7 +137,7 @@ _SIGNATURES = {
     "packed": {
         "ps_kv_append_packed": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P],
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
-        "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
+        "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
         "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P, _P],
         "ps_head_logprobs_strips": [_I, _I],
@@ -1335,16 +1335,20 @@ class Ops:
                 page_stride, _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim,
                 page_size, window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, warps, _stream()), what)
             return out
+        # Two query heads of a key head in a CTA where there are CTAs enough without their second ones (us with 1 / 2, at the shares chosen: 64 x 1,024 keys,
+        # 32 heads on 8 of 128, 120 / 91; 4 x 2,000 27.8 / 22.7; 1 x 1,024 10.9 / 12.9; 16 x 2,048, 16 on 2 of 64, 27.1 / 22.0; 2 x 300 5.2 / 7.3).
+        ratio = n_heads // n_kv_heads
+        together = 2 if ratio > 1 and head_dim <= 128 and T * n_heads >= 128 else 1
         if not shares:
-            # As above, one head a CTA (us at 1, 2, 4, 8 shares: 1 x 129 keys, 12 heads of 64, 5.9, 5.5, 5.4, 6.0; 8 x 1,024 16.7, 11.7, 10.8, 13.1; 16 x 2,048, 16 heads on
-            # 2 of 64, 34.5, 31.5, 28.3, 33.3; 16 x 4,000, 32 on 8 of 128, 148, 125, 127, 154; 64 x 1,024, 12 of 64, 34.4, 34.9, 42.8, 67.4).
-            ctas, shares = T * n_heads, 1
+            # As above (us at 1, 2, 4, 8 shares: 1 x 129 keys, 12 heads of 64, 5.6, 5.0, 5.1, 5.4; 8 x 1,024 15.7, 10.9, 10.6, 11.7; 16 x 2,048, 16 heads on 2 of
+            # 64, 37.2, 23.8, 22.0, 24.5; 16 x 4,000, 32 on 8 of 128, 133, 94, 89, 103; 64 x 1,024, 12 of 64, 33.3, 32.9, 40.5, 60.5).
+            ctas, shares = T * n_kv_heads * -(-ratio // together), 1
             while shares < 8 and (ctas * shares * 2 <= 592 and shares * 2 <= keys // 64 or ctas * shares * 2 <= 1184 and shares * 2 <= keys // 512):
                 shares *= 2
         _check(self._packed_library().ps_packed_tokens_simt(
             _ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(out.dtype), _ptr(k_pool), _ptr(v_pool), n_pages, page_stride,
             _ptr(token_row), _ptr(positions), _ptr(block_table), block_table.shape[1], T, n_heads, n_kv_heads, head_dim, page_size,
-            window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, self.code, _stream()), what)
+            window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, together, self.code, _stream()), what)
         return out
 
     UNPACKED_BYTES = 512 << 20        # most scratch that prompts take whose rows are unpacked first (but one item's rows always)

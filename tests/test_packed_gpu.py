@@ -203,6 +203,29 @@ def test_long_contexts_and_many_tokens(dtype, tokens, length):
         assert ((out.cpu().double().view(tokens, heads, dim) - want).abs() <= limit).all()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (8, 2), (5, 1)])
+@pytest.mark.parametrize("window,softcap,with_sink", [(None, None, False), (20, 3.0, True)])
+def test_many_tokens_of_grouped_heads_in_float32(dim, heads, kv_heads, window, softcap, with_sink):
+    """Two query heads of a key head at a time, and one that is left."""
+    ops, page, tokens = ops_for(F32), 16, 30
+    lengths = [1 + 13 * i % 90 for i in range(tokens)]
+    case = PackedCase(lengths, kv_heads, dim, page, F32, seed=dim)
+    _, planes = on_device(case)
+    g = torch.Generator().manual_seed(heads)
+    q = torch.randn(tokens, heads * dim, generator=g)
+    sink = torch.randn(heads, generator=g) if with_sink else None
+    out = torch.full((tokens, heads * dim), 7.0, device=DEV)
+    at = [length - 1 for length in lengths]
+    ops.packed_attention_tokens(q.to(DEV), out, *planes, ints(range(tokens)), ints(at), case.table.to(DEV), heads, kv_heads, dim, page, window, 0.125, 90,
+                                softcap=softcap, sink=None if sink is None else sink.to(DEV))
+    held_k, held_v = case.held()
+    for i in range(tokens):
+        want, weighted, sizes = attention(q[i:i + 1].double().view(1, heads, dim), case.context(i, held_k), case.context(i, held_v), torch.tensor([at[i]]), 0.125,
+                                          window, softcap, sink)
+        assert ((out[i:i + 1].cpu().double().view(1, heads, dim) - want).abs() <= bound_of(want, weighted, sizes, 0.125, F32, 0.0, dim)).all()
+
+
 @pytest.mark.parametrize("shares,warps", [(1, 4), (1, 8), (2, 8), (4, 8), (8, 4), (8, 8)])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 32), (6, 2, 64), (3, 3, 96), (8, 1, 128), (20, 2, 128)])
 def test_shares_and_warps_of_single_tokens(shares, warps, heads, kv_heads, dim):
