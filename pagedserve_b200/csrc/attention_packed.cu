@@ -5,16 +5,18 @@
 //   q . k = sum over j of step_j (q_j . c_j) + low_j sum(q_j)           (q_j, c_j: the numbers and codes of group j)
 // and the weighted values are sum over keys of (p step_j) c + sum over keys of p low_j: a code is met by one multiply-add, the group's two numbers once a key.
 // A code is put into the mantissa of a power of two (a value's into that of 16, by a rotation and a mask; two of a key's into those of 2^23, by a byte
-// permutation each, for packed additions and multiply-adds) and moved to the middle of its range, c - 8, with low_j + 8 step_j in place of low_j: sums of 16 + c, eight times as large, cost the float32 results a digit (5 tokens, 512 keys, heads of 64: 2.4e-6 off, so
-// 3e-7).  Scores, weights, sums: float32.
+// permutation each, for packed additions and multiply-adds) and moved to the middle of its range, c - 8, with low_j + 8 step_j in place of low_j:
+// sums of 16 + c, eight times as large, cost the float32 results a digit (5 tokens, 512 keys, heads of 64: 2.4e-6 off, so 3e-7).  Scores, weights,
+// sums: float32.
 //
-// A CTA has a token, a head (or two that share a key head, whose codes it then takes apart once) and a share of its keys: tiles of 32 keys aligned to absolute positions, one tile after another for each
-// warp.  For the scores a lane has a key, for the values the numbers `lane` of every group.  The shares of a token and head are a
+// A CTA has a token, a head (or two that share a key head, whose codes it then takes apart once) and a share of its keys: tiles of 32 keys aligned
+// to absolute positions, one tile after another for each warp.  For the scores a lane has a key, for the values the numbers `lane` of every group.  The shares of a token and head are a
 // thread-block cluster and merge through shared memory, in the order of the shares.
 //
 // What bounds it: instructions, two to four for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
-// heads of 64, capped scores, a sink: 8.3 us for 3.2 MB; 64 tokens of 1,024 keys, 12 heads of 64, 33), and for few tokens the chain of page, keys, weights and values of a tile: the values of
-// 16 keys (2 groups a head) are on their way while the scores are formed (one token of 32,768 keys 56 us; with four at a time, asked for when they are due, 101).
+// heads of 64, capped scores, a sink: 8.3 us for 3.2 MB; 64 tokens of 1,024 keys, 12 heads of 64, 33), and for few
+// tokens the chain of page, keys, weights and values of a tile: the values of 16 keys (2 groups a head) are on their way while the scores are formed (one
+// token of 32,768 keys 56 us; with four at a time, asked for when they are due, 101).
 #include "packed.cuh"
 
 namespace ps {
@@ -246,8 +248,8 @@ template <typename T, int NG, int R>
 int launch_tokens(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
                   long long page_stride, const int* token_row, const int* positions, const Pages& pages, int tokens, int n_heads, int n_kv_heads,
                   int head_dim, int window, float scale, float softcap, const float* sink, int shares, cudaStream_t s) {
-    return launch_pdl_cluster(tokens_kernel<T, NG, R>, dim3(tokens, n_kv_heads * ((n_heads / n_kv_heads + R - 1) / R), shares), dim3(WARPS * 32), 0, s, shares, (const T*)q, q_stride, out,
-                              out_stride, wide, (const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, token_row, positions, pages,
+    return launch_pdl_cluster(tokens_kernel<T, NG, R>, dim3(tokens, n_kv_heads * ((n_heads / n_kv_heads + R - 1) / R), shares),
+                              dim3(WARPS * 32), 0, s, shares, (const T*)q, q_stride, out, out_stride, wide, (const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, token_row, positions, pages,
                               n_heads, n_kv_heads, head_dim, window, scale, softcap, sink);
 }
 

@@ -16,12 +16,13 @@
 // right.
 // Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each.
 //
-// What bounds it: per 128 keys and 256 queries the rows' instructions (about 2,500 clocks, 2,048 of them exponentials) at head size 64, the makers' (1,250 for
-// the keys and as much for the values) at 128; and about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
+// What bounds it: per 128 keys and 256 queries the rows' instructions (about 2,500 clocks, 2,048 of them exponentials) at head size 64, the makers' (about
+// 2,500, keys and values) at 128; and about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
 // codes) and the first passes through everything. Two prompts of 1,024 (12 heads of 64) 25.6 us; three portions of 683 and fewer queries
 // behind up to 8,192 keys (16 heads on 4 of 128) 170 us, 0.62 PFLOP/s. The way there at those two: an MMA issued behind `lane == 0`, or predicated, takes 70 to 97
 // clocks, behind elect.sync 45 (190 -> 182 us at head size 128, one query tile 68 -> 54); the queries by the rows' warps, which wait anyway, instead of the
-// makers (26.8 -> 25.6, 182 -> 170). Two threads a row, 32 scores each, were slower (30 us, 190): a meeting of the two each half, and 80 registers a thread.
+// makers (26.8 -> 25.6, 182 -> 170). Two threads a row, 32 scores each, were slower (30 us, 190: a meeting of the two each half, and 80 registers a thread), and so were six
+// makers with halves of rows (27, 211: the groups' numbers twice, a page for each).
 #include <type_traits>
 
 #include "packed.cuh"
@@ -593,7 +594,8 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
                 base_m = fresh;
                 if (moves) limit = fresh + HEADROOM;
                 l_run *= corr;
-                if (n > 0) {                                       // no P V may be under way: that of the half before has to be done (that of the one before it is: this half's scores followed it)
+                // No P V may be under way: that of the half before has to be done (that of the one before it is: this half's scores followed it).
+                if (n > 0) {
                     if (!mbar_wait(&o_done[x], (n - 1) & 1, abort_flag)) { ok = false; if (lane == 0) atomicExch(status, 60); break; }
                     tc_fence_after();
 #pragma unroll 1

@@ -1243,7 +1243,8 @@ class Ops:
         """Round this step's K/V rows ([T, n_kv_heads * head_dim] views of the compute type) to 4 bits and write them into their pages:
         what :meth:`kv_append` is for a cache of the compute type.  ``k_pool`` / ``v_pool`` uint8 [pages, n_kv_heads, slab]
         (:func:`packed_slab_bytes`), ``page_stride`` in bytes.  Token t goes to row ``token_row[t]`` of ``block_table``; one with a
-        position below 0 or without a page is left out, and no two go to one place (what it holds then is neither's).  ``k_src`` or ``v_src`` None leaves that plane as it is."""
+        position below 0 or without a page is left out, and no two go to one place (what it holds then is neither's).  ``k_src`` or ``v_src`` None
+        leaves that plane as it is."""
         what = "kv_append_packed"
         given = [(name, src) for name, src in (("k", k_src), ("v", v_src)) if src is not None]
         if not given:
@@ -1264,7 +1265,8 @@ class Ops:
                   page_size, fill=False):
         """What a packed cache holds of items ``first_item ..``, as pages of the compute type: ``out`` [n_items * span / P, 2, n_kv_heads, P,
         head_dim], contiguous, P a power of two that divides ``span``.  Position p of the i-th of these items goes to page i * span / P +
-        p / P; positions from ``kv_len`` of the item (or ``span``) on are left as they are, those without a page, too, or (``fill``) become zeros.  ``item_row``: the block-table row of each item."""
+        p / P; positions from ``kv_len`` of the item (or ``span``) on are left as they are, those without a page, too, or (``fill``) become zeros.
+        ``item_row``: the block-table row of each item."""
         what = "kv_unpack"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         _require(out, "out", self.dtype)
