@@ -14,7 +14,8 @@
 // Queries are scaled row by row by a power of two, so that any bfloat16 row is one in float16. Keys and values are not: a block that meets one
 // beyond 60,000, or none beyond 2^-9, or a NaN, or a key without a page, forms its rows again in float32 from the codes (rows_again below), which is slow and
 // right.
-// Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each.
+// Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each; a block of
+// few keys takes fewer of them, and the others end at once.
 //
 // What bounds it: per 128 keys and 256 queries the rows' instructions (about 2,500 clocks, 2,048 of them exponentials) at head size 64, the makers' (about
 // 2,500, keys and values) at 128; and about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __restrict__ out, long long out_stride, Cache cache,
                const int* __restrict__ q_start, const int* __restrict__ kv_len, const int* __restrict__ item_row, int n_items, int n_heads,
                int n_kv_heads, int head_dim, int window, float scale, float softcap, SoftmaxExtras extras, int aligned_q, int aligned_out,
-               int* __restrict__ status) {
+               int most, int* __restrict__ status) {
     using L = Layout<HD>;
     constexpr int KV_STAGES = L::KV_STAGES, GROUPS_MOST = HD / GROUP;
     extern __shared__ unsigned char smem_raw[];
@@ -280,14 +281,15 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         block -= blocks;
     }
     if (item < 0) return;
-    const int h = blockIdx.x, g = h / (n_heads / n_kv_heads), share = blockIdx.z, shares = gridDim.z;
+    const int h = blockIdx.x, g = h / (n_heads / n_kv_heads), share = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int qs = q_start[item], q_len = q_start[item + 1] - qs;
     const int pos0 = kv_len[item] - q_len + qb * 2 * BQ;              // position of the block's first query
     const int rows = min(2 * BQ, q_len - qb * 2 * BQ), tok0 = qs + qb * 2 * BQ;
     const int hi = pos0 + rows - 1, lo = pos0 < 0 ? 0 : first_visible_key(pos0, window);
-    // the share's run of the block's key tiles
-    const int kb_all = lo / BKEY, kb_count = max(hi, 0) / BKEY - kb_all + 1;
+    // the share's run of the block's key tiles: `most` of them or fewer, while the cluster's CTAs last; one without a share is done
+    const int kb_all = lo / BKEY, kb_count = max(hi, 0) / BKEY - kb_all + 1, shares = min((int)gridDim.z, (kb_count + most - 1) / most);
+    if (share >= shares) return;
     const int kb_first = kb_all + kb_count * share / shares, kb_last = kb_all + kb_count * (share + 1) / shares - 1;
     // those of them that a query tile's rows see (a second tile without rows: none)
     auto first_of = [&](int x) {
@@ -725,7 +727,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
 template <int HD, bool CAPPED>
 int launch(const void* q, long long q_stride, void* out, long long out_stride, int wide, const Cache& cache, const int* q_start, const int* kv_len,
            const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
-           const float* sink, int shares, int* status, cudaStream_t s) {
+           const float* sink, int shares, int most, int* status, cudaStream_t s) {
     auto kernel = prompts_kernel<HD, CAPPED>;
     static size_t raised[MAX_DEVICES] = {0};
     if (!ensure_dynamic_smem((const void*)kernel, Layout<HD>::SMEM, raised)) return PS_ERR_LAUNCH;
@@ -733,7 +735,7 @@ int launch(const void* q, long long q_stride, void* out, long long out_stride, i
     const int aligned_out = !((uintptr_t)out & 15) && out_stride % 8 == 0 && head_dim % 8 == 0;
     return launch_pdl_cluster(kernel, dim3(n_heads, max_blocks, shares), dim3(THREADS), Layout<HD>::SMEM, s, shares, (const __nv_bfloat16*)q, q_stride, out, out_stride, cache,
                       q_start, kv_len, item_row, n_items, n_heads, n_kv_heads, head_dim, window, scale, softcap, softmax_extras(scale, softcap, sink, wide),
-                      aligned_q, aligned_out, status);
+                      aligned_q, aligned_out, most, status);
 }
 
 }  // namespace packedtc
@@ -741,20 +743,20 @@ int launch(const void* q, long long q_stride, void* out, long long out_stride, i
 
 // q / out: the step's flat rows of n_heads * head_dim numbers; item i's tokens are rows q_start[i] .. q_start[i + 1], the last ones of kv_len[i], its
 // pages row item_row[i] of block_table (bt_stride wide).  max_blocks >= sum over the items of ceil(tokens / 256).  wide: out is float32.
-// shares: CTAs (a cluster) that share a block's keys out, 1, 2, 4 or 8.
+// shares: CTAs (a cluster) that share a block's keys out, 1, 2, 4 or 8; most: tiles of 128 keys from which on a block takes another of them.
 PS_EXPORT int ps_packed_prompts_tc(const void* q, long long q_stride, void* out, long long out_stride, int wide, const void* k_pool, const void* v_pool,
                                    int n_pages, long long page_stride, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
                                    const int* item_row, int n_items, int max_blocks, int n_heads, int n_kv_heads, int head_dim, int page_size,
-                                   int window, float scale, float softcap, const float* sink, int shares, int* status, void* stream) {
+                                   int window, float scale, float softcap, const float* sink, int shares, int most, int* status, void* stream) {
     using namespace ps::packedtc;
     if (n_items <= 0 || max_blocks <= 0) return PS_OK;
     if (!q || !out || !k_pool || !v_pool || !q_start || !kv_len || !block_table || !status) return PS_ERR_BAD_ARGUMENT;
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_blocks > 65535) return PS_ERR_BAD_ARGUMENT;
     if (!ps::packed::sizes_ok(n_kv_heads, head_dim, page_size) || head_dim > 128) return PS_ERR_UNSUPPORTED;
-    if (shares != 1 && shares != 2 && shares != 4 && shares != 8) return PS_ERR_BAD_ARGUMENT;
+    if ((shares != 1 && shares != 2 && shares != 4 && shares != 8) || most <= 0) return PS_ERR_BAD_ARGUMENT;
     if (page_stride % 16 || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) return PS_ERR_UNSUPPORTED;
     const Cache cache = {(const unsigned char*)k_pool, (const unsigned char*)v_pool, page_stride, {block_table, bt_stride, n_pages, ps::packed::log2_of(page_size)}};
     auto run = head_dim <= 64 ? (softcap > 0.f ? launch<64, true> : launch<64, false>) : (softcap > 0.f ? launch<128, true> : launch<128, false>);
     return run(q, q_stride, out, out_stride, wide, cache, q_start, kv_len, item_row, n_items, max_blocks, n_heads, n_kv_heads, head_dim, window, scale,
-               softcap, sink, shares, status, (cudaStream_t)stream);
+               softcap, sink, shares, most, status, (cudaStream_t)stream);
 }

@@ -139,7 +139,7 @@ _SIGNATURES = {
         "ps_kv_unpack": [_P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "ps_packed_tokens_simt": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _I, _P],
         "ps_packed_tokens_mma": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P],
-        "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _P, _P],
+        "ps_packed_prompts_tc": [_P, _L, _P, _L, _I, _P, _P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _I, _I, _P, _P],
         "ps_head_logprobs_strips": [_I, _I],
         "ps_head_logprobs": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P],
         "ps_token_logprobs": [_P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
@@ -1390,19 +1390,15 @@ class Ops:
         if self.dtype == torch.bfloat16:
             # (an entry of b blocks of 64 queries has at most (b + 3) / 4 of 256)
             blocks = (max_blocks + 3 * n_items) // 4
+            most = 1
             if not shares:
-                # Shares pay where they leave every CTA an SM, from two tiles of 128 keys each on (us at 1, 2, 4 shares: 128 queries behind 3,872
-                # keys, 12 heads of 64, 68.4, 41.3, 26.5; 256 behind 744 24.7, 20.7, 17.9; two prompts of 1,024 27.6, 31.1, 51.4).
-                keys = min(int(max_kv_len), abs(window) + 255) if window else int(max_kv_len)
-                shares = 1
-                while shares < 8 and n_heads * blocks * shares * 2 <= 148 and shares * 2 <= keys // 256:
-                    shares *= 2
+                shares, most = self._prompt_shares(n_items, blocks, max_blocks * 64, int(max_kv_len), abs(window or 0), n_heads)
             self.launches += 1
             _check(self._packed_library().ps_packed_prompts_tc(
                 _ptr(q), q.stride(0), _ptr(out), out.stride(0), 1 if out.dtype is torch.float32 else 0, _ptr(k_pool), _ptr(v_pool), n_pages,
                 page_stride, _ptr(q_start) + 4 * first_item, _ptr(kv_len) + 4 * first_item, _ptr(block_table), block_table.shape[1],
                 _ptr(item_row) + 4 * first_item, n_items, blocks, n_heads, n_kv_heads, head_dim, page_size, window or 0, scale,
-                float(softcap or 0.0), _ptr(sink), shares, _ptr(self.status_flag(device)), _stream()), what)
+                float(softcap or 0.0), _ptr(sink), shares, most, _ptr(self.status_flag(device)), _stream()), what)
             return out
         # float32: the rows as pages of the compute type, some items at a time, and the kernels for those.
         page = 64
@@ -1419,6 +1415,26 @@ class Ops:
             self._prompts_from_pages(q, out, scratch, q_start[start:], kv_len[start:], table, counting, count, max_blocks, n_heads, n_kv_heads,
                                      head_dim, page, window, scale, softcap, sink)
         return out
+
+    @staticmethod
+    def _prompt_shares(n_items, blocks, queries, longest, extent, n_heads):
+        """(CTAs of a cluster, key tiles from which on a block takes another of them): shares pay while each CTA has an SM of its own, from two tiles
+        each on.  Blocks of items alike in length are counted.
+
+        us without / with: 128 queries behind 3,872 keys, 12 heads of 64, 49.1 / 18.2; 256 behind 744 22.8 / 16.8; a prompt of 2,048 36.7 / 32.8; two of
+        1,024 26.2 / 25.9; one of 1,024 with 25 heads, 150 CTAs with them, 22.4 / 28.0."""
+        shares, most = 1, -(-longest // 128) + 1
+        if n_heads * blocks > 148:
+            return shares, most
+        each = -(-queries // n_items)                              # queries of an item
+        seen = lambda end: min(end, extent + 255 if extent else end)
+        tiles = [-(-seen(longest - each + min(each, 256 * (i + 1))) // 128) for i in range(-(-each // 256))]
+        for more in (2, 4, 8):
+            least = -(-max(tiles) // more)
+            if least < 2 or n_heads * n_items * sum(min(more, -(-count // least)) for count in tiles) > 148:
+                break
+            shares, most = more, least
+        return shares, most
 
     def packed_prompts_ok(self, q, out, head_dim, max_blocks):
         """Whether :meth:`packed_attention_prompts` takes these rows: heads of up to 128 numbers, in float32 in whole 16-byte pieces."""
