@@ -107,3 +107,16 @@ def test_declared_arguments_are_the_sources():
         for entry in re.finditer(r"PS_EXPORT int (\w+)\(([^)]*)\)", text):
             found[entry[1]] = "".join("P" if "*" in part else "L" if "long long" in part else "F" if "float" in part else "I" for part in entry[2].split(","))
     assert found == {name: "".join(kinds[kind] for kind in arguments) for name, arguments in declared.items()}
+
+
+def test_shares_of_prompts():
+    """Clusters only while every CTA has an SM of its own, and no share of fewer than two tiles."""
+    from pagedserve_b200.kernels.ops import Ops
+
+    for n_items, queries, longest, extent, heads in ((1, 64, 64, 0, 12), (1, 128, 4000, 0, 12), (2, 2048, 1024, 0, 12), (1, 1024, 1024, 0, 25), (3, 2048, 8192, 0, 16),
+                                                     (1, 64, 1, 0, 1), (5, 64, 70, 20, 3), (1, 64, 10 ** 6, 0, 8), (1, 64, 10 ** 6, 100, 8), (200, 12800, 64, 0, 64)):
+        blocks = (queries // 64 + 3 * n_items) // 4
+        shares, most = Ops._prompt_shares(n_items, blocks, queries, longest, extent, heads)
+        assert shares in (1, 2, 4, 8) and most >= 1
+        assert shares == 1 or (most >= 2 and heads * blocks <= 148)
+    assert Ops._prompt_shares(1, 1, 128, 4000, 0, 12) == (8, 4) and Ops._prompt_shares(1, 4, 1024, 1024, 0, 25)[0] == 1
