@@ -3,17 +3,19 @@
 //
 // One CTA per (block of 256 query tokens of one request, head, share of the keys), tiles of 128 keys aligned to absolute positions. The block is two
 // tiles of 128 queries that take turns: while the rows of one form their weights, the tensor cores work for the other.
-//   warps 0..3   a key and its value a thread: codes and scales come to registers ahead of their tile, become low + code * step (one rounding to float16,
-//                2^-12 of the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact as
-//                its own) and go to the swizzled tile, 16 bytes a word of codes
+//   warps 0..3   a key and its value a thread: codes and scales come to registers ahead of their tile, become 32 (low + code * step) (one rounding to
+//                float16, 2^-11 of the number, an eighth of bfloat16's: two bfloat16 roundings, of keys and of values, made the result twice as inexact
+//                as its own) and go to the swizzled tile, 16 bytes a word of codes
 //   warps 4, 13  issue of S = Q K^T and O += P V for the first and the second query tile (4: TMEM allocation, too)
 //   warps 5..12  a thread per query row: the query to its tile, then softmax: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves,
 //                and O with it, only when a score is beyond it by 2^8, which float16 has room for
 // A tile's keys go through in two halves of 64, whose scores have columns of their own: P of a half takes the place of its scores, P V of the half is
 // issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half.
-// Queries are scaled row by row by a power of two, so that any bfloat16 row is one in float16. Keys and values are not: a block that meets one
-// beyond 60,000, or none beyond 2^-9, or a NaN, or a key without a page, forms its rows again in float32 from the codes (rows_again below), which is slow and
-// right.
+// Queries are scaled row by row by a power of two, which leaves a number of a bfloat16 row as it is, or within 2^-33 of the row's largest: 2^-13 of any group whose
+// largest is 2^-20 of that. Keys and values are all scaled by 2^5, which puts ordinary ones into the middle of float16's range. A step or a low of 2^-22 or more
+// (2^-17 once scaled) is a float16 number then, of eight digits on a grid of 2^-24, and so low + code * step, on that grid too, is rounded to 2^-11 of itself or not at
+// all. A block that needs a group with a smaller step or low other than zero, with a number beyond 1,875 (60,000 once scaled) or a NaN, a key without a page, or a query
+// with a smaller group other than zero, forms its rows again in float32 from the codes (rows_again below), which is slow and right.
 // Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each; a block of
 // few keys takes fewer of them, and the others end at once.
 //
@@ -35,7 +37,8 @@ using namespace packed;
 
 constexpr int BQ = 128, BKEY = 128, MAKERS = 128, THREADS = MAKERS + 64 + 2 * BQ;
 constexpr uint64_t WAIT_LIMIT_NS = 200ull * 1000 * 1000;
-constexpr float MOST = 60000.f, LEAST = 0.001953125f;              // sizes of numbers that float16 holds to 2^-12 of the largest
+constexpr float CACHE_SCALE = 32.f, MOST = 60000.f;                // what keys and values are multiplied by on their way into float16; the largest there
+constexpr uint32_t LEAST_BITS = 0x3480u;                           // 2^-22 in bfloat16: steps and lows from there on are float16 numbers once scaled
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint64_t timer_ns() {
@@ -268,7 +271,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     uint64_t* o_full = o_done + 2;            // [2] MMA -> rows: O is complete (o_done could be a phase or two behind where no one waited for it)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* sizes_s = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(bars) + 256);      // largest key, largest value (bits), whether something is strange
+    uint32_t* strange_s = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(bars) + 256);    // whether the rows are to be formed again
 
     pdl_prologue();
     q = pdl_fresh(q);
@@ -316,7 +319,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             mbar_init(&o_done[x], 1);
             mbar_init(&o_full[x], 1);
         }
-        sizes_s[0] = sizes_s[1] = sizes_s[2] = 0u;
+        *strange_s = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 4) {
@@ -366,7 +369,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         uint4 k_codes[GROUPS_MOST], v_codes[GROUPS_MOST];
         uint32_t k_scales[GROUPS_MOST], v_scales[GROUPS_MOST];
         bool strange = false;
-        float k_most = 0.f, v_most = 0.f;
+        uint32_t least = 0xffffffffu;                              // the smallest step and low other than 0 (bits of their sizes, less 1), either in its half
         long long page_at = -1;                                    // of the key whose numbers are asked for (below 0: not needed, or no page)
         int page_row = 0;
         // A key's entry of the block table is asked for a tile before its codes, and not looked at until then: a comparison would wait for it.
@@ -394,13 +397,13 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             }
         };
         // a row of a tile: place p of the codes (part p / groups of group p % groups) becomes eight numbers; what is not there becomes zeros
-        auto make = [&](unsigned char* tile, const uint4 (&codes)[GROUPS_MOST], const uint32_t (&scales)[GROUPS_MOST], float& most_size) {
+        auto make = [&](unsigned char* tile, const uint4 (&codes)[GROUPS_MOST], const uint32_t (&scales)[GROUPS_MOST]) {
             uint32_t step[GROUPS_MOST], low[GROUPS_MOST];
 #pragma unroll
             for (int j = 0; j < GROUPS_MOST; ++j) {
-                const float a = step_of(scales[j]), b = low_of(scales[j]), size = fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b)));
-                strange |= !(size <= MOST);
-                most_size = fmaxf(most_size, size);
+                const float a = step_of(scales[j]) * CACHE_SCALE, b = low_of(scales[j]) * CACHE_SCALE;
+                strange |= !(fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b))) <= MOST);
+                least = __viaddmin_u16x2(scales[j] & 0x7fff7fffu, 0xffffffffu, least);         // (0 less 1 is the largest of all)
                 step[j] = half_pair(a, a);
                 low[j] = half_pair(b, b);
             }
@@ -434,21 +437,16 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             unsigned char* tile = kv_s + (size_t)s * L::STAGE_BYTES;
             if (kb < kb_last) locate(kb + 1);
             if (!mbar_wait(&k_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 51); break; }
-            make(tile, k_codes, k_scales, k_most);
+            make(tile, k_codes, k_scales);
             arrive(&k_full[s]);
             if (kb < kb_last) fetch(cache.k_pool, k_codes, k_scales);
             if (!mbar_wait(&v_empty[s], free, abort_flag)) { if (lane == 0) atomicExch(status, 52); break; }
-            make(tile + L::KV_BYTES, v_codes, v_scales, v_most);
+            make(tile + L::KV_BYTES, v_codes, v_scales);
             arrive(&v_full[s]);
             if (kb < kb_last) fetch(cache.v_pool, v_codes, v_scales);
         }
-        const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_most)), v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_most));
-        const bool any = __any_sync(0xffffffffu, strange);
-        if (lane == 0) {
-            atomicMax(&sizes_s[0], k_bits);
-            atomicMax(&sizes_s[1], v_bits);
-            if (any) atomicExch(&sizes_s[2], 1u);
-        }
+        strange |= (least & 0xffffu) < LEAST_BITS - 1u || (least >> 16) < LEAST_BITS - 1u;
+        if (__any_sync(0xffffffffu, strange) && lane == 0) atomicExch(strange_s, 1u);
     } else if (warp == 4 || warp == 13) {
         // ------------------------------------------------ MMA issuers, one for each query tile
         // D f32, A/B f16: S = Q K^T both K-major, N = 64; O = P V with A from TMEM and B MN-major (bit 16), N = HD
@@ -523,7 +521,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         float factor;
         {
             const __nv_bfloat16* row = q + (long long)(tok0 + place) * q_stride + (long long)h * head_dim;
-            float most = 0.f;
+            float most = 0.f, group_most[GROUPS_MOST];
             bool odd = false;
             uint4 raw[HD / 8];                                     // the whole row at once: its loads are under way together
 #pragma unroll
@@ -542,17 +540,25 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
                 const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                float& largest = group_most[i / 4];
+                if (i % 4 == 0) largest = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float lo_half = fabsf(__uint_as_float(w[j] << 16)), hi_half = fabsf(__uint_as_float(w[j] & 0xffff0000u));
-                    most = max3(most, lo_half, hi_half);
+                    largest = max3(largest, lo_half, hi_half);
                     odd |= !(lo_half <= 3.4028235e38f) || !(hi_half <= 3.4028235e38f);
                 }
             }
+#pragma unroll
+            for (int j = 0; j < GROUPS_MOST; ++j) most = fmaxf(most, group_most[j]);
+            bool small = false;
+#pragma unroll
+            for (int j = 0; j < GROUPS_MOST; ++j) small |= group_most[j] > 0.f && group_most[j] < most * 0x1p-20f;
+            if (small && !odd) *strange_s = 1u;
             // 2^up brings the largest to [256, 512); a NaN or infinity stays one
-            const int up = most > 0.f && !odd ? min(126, 135 - max(1, (int)(__float_as_uint(most) >> 23))) : 0;
+            const int up = most > 0.f && !odd ? min(121, 135 - max(1, (int)(__float_as_uint(most) >> 23))) : 0;
             const float by = __uint_as_float((uint32_t)(127 + up) << 23);
-            factor = __uint_as_float((uint32_t)(127 - up) << 23);
+            factor = __uint_as_float((uint32_t)(127 - up) << 23) * (1.f / CACHE_SCALE);      // (of queries and keys; up is -119 to 121)
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
                 const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -646,7 +652,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             part_m[place] = limit > -INFINITY ? base_m : -INFINITY;
             part_l[place] = l_run;
         }
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        const float inv = l_run == 0.f ? 0.f : 1.f / (CACHE_SCALE * l_run);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
             uint32_t orr[16];
@@ -678,18 +684,13 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)L::TMEM_COLS) : "memory");
     }
-    float k_most = __uint_as_float(sizes_s[0]), v_most = __uint_as_float(sizes_s[1]);
-    uint32_t strange = sizes_s[2];
+    uint32_t strange = *strange_s;
     if (shares > 1) {
         __syncwarp();
         cluster_sync_all();
-        for (int other = 0; other < shares; ++other) {
-            k_most = fmaxf(k_most, __uint_as_float(ld_cluster_u32(&sizes_s[0], other)));
-            v_most = fmaxf(v_most, __uint_as_float(ld_cluster_u32(&sizes_s[1], other)));
-            strange |= ld_cluster_u32(&sizes_s[2], other);
-        }
+        for (int other = 0; other < shares; ++other) strange |= ld_cluster_u32(strange_s, other);
     }
-    if (strange || (k_most > 0.f && k_most < LEAST) || (v_most > 0.f && v_most < LEAST)) {
+    if (strange) {
         rows_again(q, q_stride, out, out_stride, extras.wide, cache, table_row, head_at, h, head_dim, tok0, pos0, rows, window, scale, softcap, extras.sink,
                    share * (THREADS / 32) + warp, shares * (THREADS / 32), lane);
     } else if (shares > 1) {
@@ -712,7 +713,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = fmaf(one[j], by, v[j]);
             }
-            const float inv = total == 0.f ? 0.f : 1.f / total;
+            const float inv = total == 0.f ? 0.f : 1.f / (CACHE_SCALE * total);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] *= inv;
             store8(place, d, v);

@@ -1,0 +1,93 @@
+"""Attention over a cache held in 4 bits where numbers of very different sizes meet: groups, rows and weights far below others."""
+
+import pytest
+import torch
+
+from plain_packed import PackedCase, attention
+from test_packed_gpu import BF16, DEV, F32, bound_of, ints, on_device, ops_for
+
+pytestmark = pytest.mark.gpu
+
+
+def prompts(ops, case, planes, q, new, heads, scale, shares=0, window=None, softcap=None, sink=None):
+    length, kv_heads, dim = case.lengths[0], case.kv_heads, case.dim
+    out = torch.full((new, heads * dim), 7.0, dtype=q.dtype, device=DEV)
+    ops.packed_attention_prompts(q.to(DEV), out, *planes, ints([0, new]), ints([length]), case.table.to(DEV), ints([0]), 0, 1, -(-new // 64), length, heads, kv_heads, dim,
+                                 case.page, window, scale, softcap=softcap, sink=None if sink is None else sink.to(DEV), shares=shares)
+    return out.cpu().double().view(new, heads, dim)
+
+
+def tokens(ops, case, planes, q, positions, heads, scale, shares=0, window=None, softcap=None, sink=None):
+    kv_heads, dim = case.kv_heads, case.dim
+    out = torch.full((len(positions), heads * dim), 7.0, dtype=q.dtype, device=DEV)
+    ops.packed_attention_tokens(q.to(DEV), out, *planes, ints([0] * len(positions)), ints(positions), case.table.to(DEV), heads, kv_heads, dim, case.page, window, scale,
+                                case.lengths[0], softcap=softcap, sink=None if sink is None else sink.to(DEV), shares=shares)
+    return out.cpu().double().view(len(positions), heads, dim)
+
+
+def limit_of(found, scale, dtype, dim):
+    """(bfloat16: keys, values and weights of prompts in float16, half a step of 2^-11 each; weights times steps of single tokens likewise)"""
+    return bound_of(*found, scale, dtype, *((2.0 ** -10, dim, 2.0 ** -11) if dtype == BF16 else (2.0 ** -20, dim)))
+
+
+def agrees(got, found, limit):
+    off = ((got - found[0]).abs() / limit).max()
+    assert off <= 1, float(off)
+
+
+def shrunk(case, what, size):
+    """Numbers of ``size`` beside ordinary ones; what the queries are to be multiplied by, or None."""
+    if what == "a group of values":
+        case.v[:, 0, :32] *= size
+    elif what == "a group of one value":
+        case.v[:, -1, :32] = size
+    elif what == "the first rows' values":
+        case.v[:40] *= size
+    elif what == "a channel":
+        case.v[:, 0, :32] = case.v[:, 0, :32].abs() + 0.125
+        case.v[:, 0, 5] = size                                             # the least of its group: code 0
+    elif what == "a group of keys":
+        case.k[:, 0, :32] *= size
+        return 1 / size
+    elif what == "the last values":
+        case.v[-20:] *= size
+    return None
+
+
+def beside_ordinary_ones(dtype, size, what, heads, kv_heads, dim, new):
+    length = new if what == "the first rows' values" else 700             # (so that some queries see nothing else)
+    case = PackedCase([length], kv_heads, dim, 16, dtype, seed=dim)
+    grown = shrunk(case, what, size)
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    q = torch.randn(new, heads, dim, generator=torch.Generator().manual_seed(3))
+    if grown is not None:
+        q[:, :heads // kv_heads, :32] *= grown
+    q = q.flatten(1).to(dtype)
+    positions, scale = torch.arange(length - new, length), dim ** -0.5
+    return ops_for(dtype), case, planes, q, positions, scale, attention(q.double().view(new, heads, dim), k, v, positions, scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1e-4, 1e-5, 1e-6, 3e-8, 1e-12])
+@pytest.mark.parametrize("what", ["a group of values", "a group of one value", "the first rows' values", "a channel", "a group of keys", "the last values"])
+@pytest.mark.parametrize("heads,kv_heads,dim,shares", [(2, 2, 64, 1), (4, 2, 128, 8), (3, 1, 40, 1), (2, 2, 96, 2)])
+def test_small_numbers_in_prompts(dtype, size, what, heads, kv_heads, dim, shares):
+    """What is held of a small group, row or channel reaches the result to the same relative error as ordinary numbers."""
+    new = 300
+    ops, case, planes, q, positions, scale, found = beside_ordinary_ones(dtype, size, what, heads, kv_heads, dim, new)
+    agrees(prompts(ops, case, planes, q, new, heads, scale, shares=shares if dtype == BF16 else 0), found, limit_of(found, scale, dtype, dim))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(12, 12, 64), (8, 2, 128)])
+def test_results_repeat_bit_by_bit(heads, kv_heads, dim):
+    ops, length, new = ops_for(BF16), 900, 300
+    case = PackedCase([length], kv_heads, dim, 16, BF16, seed=1)
+    _, planes = on_device(case)
+    q = torch.randn(new, heads * dim, generator=torch.Generator().manual_seed(3)).bfloat16()
+    for shares in (0, 1, 4):
+        one, two = (prompts(ops, case, planes, q, new, heads, 0.125, shares=shares) for _ in range(2))
+        assert torch.equal(one, two)
+        at = list(range(length - 8, length))
+        one, two = (tokens(ops, case, planes, q[:8], at, heads, 0.125, shares=shares) for _ in range(2))
+        assert torch.equal(one, two)
