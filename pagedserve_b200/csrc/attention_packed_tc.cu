@@ -9,6 +9,8 @@
 //   warps 4, 13  issue of S = Q K^T and O += P V for the first and the second query tile (4: TMEM allocation, too)
 //   warps 5..12  a thread per query row: the query to its tile, then softmax: maximum, weights (float16, to TMEM), sum. The base of a row's weights moves,
 //                and O with it, only when a score is beyond it by 2^8, which float16 has room for
+// Weights are 2^7 times what their base gives, so that one is held to 2^-11 of itself or to 2^-32 of its row's largest; their sum has them unrounded. A sink joins
+// the sum at the end.
 // A tile's keys go through in two halves of 64, whose scores have columns of their own: P of a half takes the place of its scores, P V of the half is
 // issued and then the scores of the same half of the next tile (MMAs run in the order of their issue), while the rows work on the other half.
 // Queries are scaled row by row by a power of two, which leaves a number of a bfloat16 row as it is, or within 2^-33 of the row's largest: 2^-13 of any group whose
@@ -183,6 +185,7 @@ struct Layout {
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
 };
 constexpr float HEADROOM = 8.f;                                     // log2 of how far a weight may be beyond 1 before its base moves
+constexpr float LIFT = 7.f;                                         // log2 of what weights are multiplied by: float16's largest is above 2^(LIFT + HEADROOM)
 
 struct Cache {
     const unsigned char* k_pool;
@@ -330,6 +333,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    const float sink_log2 = extras.sink ? extras.sink[h] * 1.4426950408889634f : -INFINITY;
     // one arrival for a whole warp
     auto arrive = [&](uint64_t* bar) {
         __syncwarp();
@@ -510,12 +514,8 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         const int lo_all = pos_last < 0 ? 0 : first_visible_key(pos_last, window);        // the first key that every row of the tile sees
         const uint32_t s_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::S_COL + x * 128;
         const uint32_t o_at = tmem_base + ((uint32_t)(quarter * 32) << 16) + L::O_COL + x * HD;
-        float base_m = 0.f, limit = -INFINITY, l_run = 0.f;        // in log2 units: the base of the weights, what a score may reach
-        if (share == 0 && extras.sink && extras.sink[h] != -INFINITY) {
-            base_m = extras.sink[h] * 1.4426950408889634f;
-            limit = base_m + HEADROOM;
-            l_run = 1.f;
-        }
+        // in log2 units: the base of the weights (of keys alone: beside a sink far above them they would be lost), what a score may reach
+        float base_m = 0.f, limit = -INFINITY, l_run = 0.f;
         bool ok = first <= last;
         // the row's query, scaled by a power of two, to its tile
         float factor;
@@ -617,8 +617,8 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
                     }
                 }
             }
-            // weights 2^(s - base)
-            const unsigned long long less = pair_of(-base_m, -base_m);
+            // weights 2^(s - base + LIFT)
+            const unsigned long long less = pair_of(LIFT - base_m, LIFT - base_m);
             unsigned long long sum_a = 0ull, sum_b = 0ull;
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
@@ -652,7 +652,7 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
             part_m[place] = limit > -INFINITY ? base_m : -INFINITY;
             part_l[place] = l_run;
         }
-        const float inv = l_run == 0.f ? 0.f : 1.f / (CACHE_SCALE * l_run);
+        const float all = extras.sink ? l_run + ex2(sink_log2 - base_m + LIFT) : l_run, inv = all == 0.f ? 0.f : 1.f / (CACHE_SCALE * all);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
             uint32_t orr[16];
@@ -700,9 +700,10 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         for (int i = threadIdx.x; i < count * PIECES; i += THREADS) {
             const int place = first + i / PIECES, d = i % PIECES * 8;
             if (d >= head_dim) continue;
-            float top = -INFINITY, total = 0.f, v[8];
+            float top = sink_log2, v[8];
             for (int other = 0; other < shares; ++other) top = fmaxf(top, ld_cluster_f32(part_m + place, other));
             const float ground = top == -INFINITY ? 0.f : top;
+            float total = extras.sink ? ex2(sink_log2 - ground + LIFT) : 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.f;
             for (int other = 0; other < shares; ++other) {

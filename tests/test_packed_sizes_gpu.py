@@ -79,6 +79,25 @@ def test_small_numbers_in_prompts(dtype, size, what, heads, kv_heads, dim, share
     agrees(prompts(ops, case, planes, q, new, heads, scale, shares=shares if dtype == BF16 else 0), found, limit_of(found, scale, dtype, dim))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shares", [1, 4])
+@pytest.mark.parametrize("sink", [10.0, 15.0, 20.0, 40.0])
+@pytest.mark.parametrize("window,softcap", [(None, None), (50, None), (None, 3.0)])
+def test_sinks_far_above_the_scores(dtype, shares, sink, window, softcap):
+    """A sink takes nearly all of a row's weight: what is left for the values is small, and right."""
+    ops, heads, dim, page, length, new = ops_for(dtype), 2, 64, 16, 600, 300
+    case = PackedCase([length], heads, dim, page, dtype, seed=5)
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    q = torch.randn(new, heads * dim, generator=torch.Generator().manual_seed(3)).to(dtype)
+    sinks, positions = torch.tensor([sink, 0.5]), torch.arange(length - new, length)
+    found = attention(q.double().view(new, heads, dim), k, v, positions, 0.125, window, softcap, sinks)
+    limit = limit_of(found, 0.125, dtype, dim)
+    extras = dict(window=window, softcap=softcap, sink=sinks, shares=shares if dtype == BF16 else 0)
+    agrees(tokens(ops, case, planes, q, positions.tolist(), heads, 0.125, **extras), found, limit)
+    agrees(prompts(ops, case, planes, q, new, heads, 0.125, **extras), found, limit)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim", [(12, 12, 64), (8, 2, 128)])
 def test_results_repeat_bit_by_bit(heads, kv_heads, dim):
     ops, length, new = ops_for(BF16), 900, 300
