@@ -6,13 +6,16 @@
 //   s   = sum over j of step_j S_j + low_j sum(q_j)
 //   O_j = (C_j - 8)^T (p step_j)               numbers x queries: again on the 16-row side; the weights turn from the first product's result
 //   o   = O_j + sum over keys of p (low_j + 8 step_j)             into the second's operand by movmatrix
-// so that keys and values are met without a rounding; a weight times its step is rounded to float16 (2^-12 of itself).
+// so that keys and values are met without a rounding; a weight times its step is rounded to float16 (2^-11 of itself).
 //   * A mask puts two codes into float16 at once: bits 4 .. 7 of a half word under the exponent of 64 are 64 + c; bits 0 .. 3 under that of 1024 are
 //     1024 + c. Keys take the first form (a shift a code), with low_j - 64 step_j in place of low_j; values take both, and one subtraction leaves
 //     c - 8: their sums are long, and what 1024 p costs in float32 would show.
-//   * Queries are scaled by a power of two to at most 512, so that any bfloat16 query is one in float16.
-//   * p step_j stays within float16 whatever the steps: p is taken relative to the largest score so far, step_j to the exponent of the group's largest
-//     one. Either moves only when a score passes the former by 2^8 or a step the latter's power of two, so that hardly a tile pays for it.
+//   * Queries are scaled by a power of two to at most 512, which leaves a bfloat16 number as it is, or within 2^-33 of its row's largest.
+//   * p step_j is at most 2^15: p is taken relative to the largest score so far, step_j to the exponent of the group's largest one less 5. Either moves only when a
+//     score passes the former by 2^8 or a step the latter's power of two, so that hardly a tile pays for it. A product is then held to 2^-11 of itself or to 2^-30
+//     of that of a weight of 1 and the largest step.
+//   * A step other than zero below 2^-19 of the largest so far (its weight may be all there is, and float16 has no digits for it), or a group of a query below 2^-17
+//     of its row: the token's heads are done again in float32 (row_again in packed.cuh), which is slow and right.
 //
 // A CTA has a token, a key head (8 or 16 of its query heads) and a share of the keys; a warp takes tiles of 16 keys, which it brings to shared
 // memory itself (cp.async, a ring of its own, no barrier). Shares are a cluster and merge through shared memory.
@@ -29,6 +32,8 @@ namespace packed {
 
 constexpr int M_KEYS = 16;
 constexpr float HEADROOM = 8.f;                            // log2 of how far a weight may be beyond 1 before its base moves
+constexpr int LIFT = 5;                                    // log2 of what products of weights and steps are multiplied by
+constexpr float LEAST_FACTOR = 6.103515625e-05f;           // 2^-14, float16's least number of eleven digits: a smaller factor of a step is not taken
 constexpr int LEAST_EXPONENT = 27, MOST_EXPONENT = 253;    // biased: steps below 2^-100 count as that, those from 2^126 on (up to 4 of it)
 
 __device__ __forceinline__ float ex2(float x) {
@@ -108,7 +113,7 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ float base_s[M_WARPS][COLUMNS], sum_s[M_WARPS][COLUMNS], share_base[COLUMNS], share_sum[COLUMNS];
     pdl_prologue();
-    q = pdl_fresh(q);
+    const __nv_bfloat16* queries = pdl_fresh(q);
     k_pool = pdl_fresh(k_pool);
     v_pool = pdl_fresh(v_pool);
     const int ratio = n_heads / n_kv_heads, blocks = (ratio + COLUMNS - 1) / COLUMNS;
@@ -124,12 +129,12 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
 
     // ---- a tile's bytes on their way. What is not visible or has no page is left as the ring holds it: its scales are not used.
     const int step_tiles = shares * M_WARPS;
-    int tile = lo / M_KEYS + share * M_WARPS + warp, ahead = tile;
+    int tile = lo / M_KEYS + share * M_WARPS + warp;
     uint32_t paged = 0;                                                          // (by_tile) the stages whose tile has a page
     // (a tile's page is asked for a tile before, and not looked at until then: a comparison here would wait for it)
     const int* table = pages.block_table + (size_t)table_row * pages.bt_stride;
     auto page_of = [&](int which) { return by_tile && which * M_KEYS <= last ? table[which * M_KEYS >> pages.page_log2] : -1; };
-    int next_page = page_of(ahead);
+    int next_page = page_of(tile);
     auto fetch = [&](int which, int stage) {
         const int key0 = which * M_KEYS, page = next_page < pages.n_pages ? next_page : -1;
         next_page = page_of(which + step_tiles);
@@ -173,18 +178,18 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     };
 #pragma unroll
     for (int s = 0; s < R::STAGES - 1; ++s) {
-        fetch(ahead, s);
-        ahead += step_tiles;
+        fetch(tile + s * step_tiles, s);
     }
 
     // ---- queries: column g of every block of eight, numbers 32 j + 8 c .. + 7, scaled to float16
     uint32_t qf[NQ][NG][4];
     float q_sum[NQ][NG][2], factor[NQ][2];                      // of columns 2 c and 2 c + 1: what this thread's scores belong to
+    uint32_t least = 0xffffffffu;                                // the smallest factor of a step other than 0, as bits
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int column = first_query + n * 8 + g;
-        const __nv_bfloat16* row = q + t * q_stride + ((long long)kv_head * ratio + column) * head_dim;
-        float x[NG][8], largest = 0.f;
+        const __nv_bfloat16* row = queries + t * q_stride + ((long long)kv_head * ratio + column) * head_dim;
+        float x[NG][8], part_largest[NG], largest = 0.f;
         bool strange = false;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
@@ -206,17 +211,22 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
                         if (d + i < head_dim) x[j][i] = __bfloat162float(row[d + i]);
                 }
             }
+            part_largest[j] = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                largest = fmaxf(largest, fabsf(x[j][i]));
+                part_largest[j] = fmaxf(part_largest[j], fabsf(x[j][i]));
                 strange |= !(fabsf(x[j][i]) <= 3.4028235e38f);
             }
+            largest = fmaxf(largest, part_largest[j]);
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             strange |= __shfl_xor_sync(0xffffffffu, (int)strange, o) != 0;
         }
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+            if (part_largest[j] > 0.f && part_largest[j] < largest * 0x1p-17f && !strange) least = 0u;
         // 2^up brings the largest to [256, 512); a NaN or infinity stays one; (exponents from 1: below are denormals, which may as well stay small)
         int up = largest > 0.f && !strange ? 135 - max(1, (int)(__float_as_uint(largest) >> 23)) : 0;
         up = min(up, 126);
@@ -248,8 +258,8 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     const float cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
 
     float base[NQ][2], limit[NQ][2], l[NQ][2], lows[NQ][NG][2], o[NQ][NG][2][4];
-    float unit_step[NG];                                         // one over the power of two of each group's largest step so far: o is in units of it
-    auto reciprocal = [](int biased) { return __uint_as_float((uint32_t)(254 - biased) << 23); };
+    float unit_step[NG];                                         // 2^LIFT over the power of two of each group's largest step so far: what o is multiplied by
+    auto reciprocal = [](int biased) { return __uint_as_float((uint32_t)(254 + LIFT - biased) << 23); };
 #pragma unroll
     for (int j = 0; j < NG; ++j) unit_step[j] = reciprocal(LEAST_EXPONENT);
 #pragma unroll
@@ -277,8 +287,7 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
         copies_wait<R::STAGES - 2>();
         __syncwarp();
         const bool whole = by_tile && (paged >> stage & 1u);
-        fetch(ahead, stage == 0 ? R::STAGES - 1 : stage - 1);                     // (the stage that the last tile was in)
-        ahead += step_tiles;
+        fetch(tile + (R::STAGES - 1) * step_tiles, stage == 0 ? R::STAGES - 1 : stage - 1);      // (the stage that the last tile was in)
         const unsigned char* at = ring + stage * R::TILE_BYTES;
         stage = stage + 1 == R::STAGES ? 0 : stage + 1;
         const int key_a = tile * M_KEYS + row_a, key_b = key_a + 8;
@@ -333,7 +342,7 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
             }
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-            moves |= fmaxf(step_of(za[j]), step_of(zb[j])) * unit_step[j] >= 4.f;        // (an exponent more than one above; false for NaN)
+            moves |= fmaxf(step_of(za[j]), step_of(zb[j])) * unit_step[j] >= (float)(4 << LIFT);        // (an exponent more than one above; false for NaN)
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -349,7 +358,7 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 const int largest = (int)(__float_as_uint(fmaxf(0.f, fmaxf(step_of(za[j]), step_of(zb[j])))) >> 23);
-                const int old = 254 - (int)(__float_as_uint(unit_step[j]) >> 23);
+                const int old = 254 + LIFT - (int)(__float_as_uint(unit_step[j]) >> 23);
                 const int fresh = max(old, min(MOST_EXPONENT, __reduce_max_sync(0xffffffffu, largest)));
                 const float shrink = __uint_as_float((uint32_t)max(0, 127 - (fresh - old)) << 23);
                 unit_step[j] = reciprocal(fresh);
@@ -404,7 +413,9 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
             const uint32_t a4 = half_add(thousand_plus(xs), LESS_1032), a5 = half_add(sixty_four_plus(xs), LESS_72),
                            a6 = half_add(thousand_plus(ys), LESS_1032), a7 = half_add(sixty_four_plus(ys), LESS_72);
             const float mid_a = fmaf(8.f, step_of(za[j]), low_of(za[j])), mid_b = fmaf(8.f, step_of(zb[j]), low_of(zb[j]));
-            const float by_a = step_of(za[j]) * unit_step[j], by_b = step_of(zb[j]) * unit_step[j];
+            // (a step of 0 gets a factor of -2^-126, which is the largest of all as bits and makes weights of 0 in float16)
+            const float by_a = fmaf(step_of(za[j]), unit_step[j], -0x1p-126f), by_b = fmaf(step_of(zb[j]), unit_step[j], -0x1p-126f);
+            least = __vimin3_u32(__float_as_uint(by_a), __float_as_uint(by_b), least);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 const uint32_t b0 = transposed(half_pair(s[n][0] * by_a, s[n][1] * by_a));
@@ -430,6 +441,7 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
                 for (int j = 0; j < NG; ++j) lows[n][j][b] += __shfl_xor_sync(0xffffffffu, lows[n][j][b], x);
             }
         }
+    const bool strange = __any_sync(0xffffffffu, least < __float_as_uint(LEAST_FACTOR));
     __syncthreads();                                             // the rings are done with
     float* acc_s = reinterpret_cast<float*>(memory);             // [M_WARPS][COLUMNS][NUMBERS]
 #pragma unroll
@@ -443,13 +455,13 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int d = j * GROUP + 8 * (g & 3) + (g >> 2) + 4 * x;
-                    const float unit = reciprocal((int)(__float_as_uint(unit_step[j]) >> 23));
+                    const float unit = __uint_as_float((254u << 23) - __float_as_uint(unit_step[j]));      // one over it
                     row[d] = fmaf(o[n][j][x][b], unit, lows[n][j][b]);
                     row[d + 2] = fmaf(o[n][j][x][2 + b], unit, lows[n][j][b]);
                 }
             if (g == 0) {
                 base_s[warp][column] = limit[n][b] == -INFINITY ? -INFINITY : base[n][b];
-                sum_s[warp][column] = l[n][b];
+                sum_s[warp][column] = strange ? __uint_as_float(0x7fffffffu) : l[n][b];         // (a NaN: the row is done again)
             }
         }
     __syncthreads();
@@ -475,10 +487,10 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
     }
     if (shares > 1) cluster_sync_all();
     else __syncthreads();
-    // the shares': each of them finishes a part of the numbers
+    // the shares': each of them finishes a part of the numbers, a warp 32 of a query at a time
     for (int i = share * M_WARPS * 32 + threadIdx.x; i < COLUMNS * NUMBERS; i += shares * M_WARPS * 32) {
         const int column = i / NUMBERS, d = i % NUMBERS, query = first_query + column;
-        if (query >= ratio || d >= head_dim) continue;
+        if (query >= ratio) continue;
         const int h = kv_head * ratio + query;
         const float sink_log2 = sink ? sink[h] * 1.4426950408889634f : -INFINITY;
         float top = sink_log2, sum = 0.f;
@@ -490,6 +502,14 @@ tokens_mma_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void*
             total = fmaf(shares > 1 ? ld_cluster_f32(&share_sum[column], x) : share_sum[column], by, total);
             sum = fmaf(shares > 1 ? ld_cluster_f32(&share_acc[i], x) : share_acc[i], by, sum);
         }
+        if (total != total) {                                     // weights that are no numbers, or that float16 does not hold
+            const Cache cache = {k_pool, v_pool, page_stride, pages};
+            if (d < GROUP)                                        // (the warp that has the query's first numbers; read anew: no register keeps them in the loop)
+                row_again(q + t * q_stride + (long long)h * head_dim, out, t * out_stride + (long long)h * head_dim, wide, cache, token_row[t],
+                          (long long)kv_head * slab_bytes(page_size, head_dim), head_dim, positions[t], window, scale, softcap, sink ? sink + h : nullptr, lane);
+            continue;
+        }
+        if (d >= head_dim) continue;
         // (no key at all: zero; a NaN stays one)
         const float result = total == 0.f ? sum * 0.f : sum / total;
         const long long to = t * out_stride + (long long)h * head_dim + d;

@@ -17,7 +17,7 @@
 // largest is 2^-20 of that. Keys and values are all scaled by 2^5, which puts ordinary ones into the middle of float16's range. A step or a low of 2^-22 or more
 // (2^-17 once scaled) is a float16 number then, of eight digits on a grid of 2^-24, and so low + code * step, on that grid too, is rounded to 2^-11 of itself or not at
 // all. A block that needs a group with a smaller step or low other than zero, with a number beyond 1,875 (60,000 once scaled) or a NaN, a key without a page, or a query
-// with a smaller group other than zero, forms its rows again in float32 from the codes (rows_again below), which is slow and right.
+// with a smaller group other than zero, forms its rows again in float32 from the codes (row_again in packed.cuh), which is slow and right.
 // Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each; a block of
 // few keys takes fewer of them, and the others end at once.
 //
@@ -186,69 +186,6 @@ struct Layout {
 };
 constexpr float HEADROOM = 8.f;                                     // log2 of how far a weight may be beyond 1 before its base moves
 constexpr float LIFT = 7.f;                                         // log2 of what weights are multiplied by: float16's largest is above 2^(LIFT + HEADROOM)
-
-struct Cache {
-    const unsigned char* k_pool;
-    const unsigned char* v_pool;
-    long long page_stride;
-    Pages pages;
-};
-
-// Rows of a block once more, in float32 from the codes, a warp a row: lane l has number 32 j + l of every group.
-__device__ __noinline__ void rows_again(const __nv_bfloat16* q, long long q_stride, void* out, long long out_stride, int wide, const Cache cache, int table_row,
-                                        long long head_at, int h, int head_dim, int tok0, int pos0, int rows, int window, float scale,
-                                        float softcap, const float* sink, int warp, int warps, int lane) {
-    const int groups = groups_of(head_dim), page_size = 1 << cache.pages.page_log2, shift = code_shift(lane & 7);
-    for (int r = warp; r < rows; r += warps) {
-        const int p = pos0 + r, last = min(p, (cache.pages.bt_stride << cache.pages.page_log2) - 1);
-        float x[4], acc[4], m = -INFINITY, l = 0.f;
-        if (sink) {
-            m = sink[h];
-            l = 1.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int d = j * GROUP + lane;
-            x[j] = d < head_dim ? __bfloat162float(q[(long long)(tok0 + r) * q_stride + (long long)h * head_dim + d]) : 0.f;
-            acc[j] = 0.f;
-        }
-        for (int key = first_visible_key(p, window); key <= last; ++key) {
-            const int page = cache.pages.of(table_row, key);
-            if (page < 0) continue;
-            const long long at = (long long)page * cache.page_stride + head_at;
-            const int row = key & (page_size - 1);
-            float s = 0.f, v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = 0.f;
-                if (j < groups) {
-                    const int word = (row * 4 + (lane >> 3)) * groups + j, scale_at = page_size * groups * 4 + row * groups + j;
-                    const uint32_t *k = reinterpret_cast<const uint32_t*>(cache.k_pool + at), *w = reinterpret_cast<const uint32_t*>(cache.v_pool + at);
-                    const bool there = j * GROUP + lane < head_dim;            // (a number that is not there has no code)
-                    if (there) s = fmaf(fmaf((float)(k[word] >> shift & 15u), step_of(k[scale_at]), low_of(k[scale_at])), x[j], s);
-                    v[j] = fmaf((float)(w[word] >> shift & 15u), step_of(w[scale_at]), low_of(w[scale_at]));
-                }
-            }
-            s = warp_sum(s) * scale;
-            if (softcap > 0.f) s = softcap * tanhf(s / softcap);
-            const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, shrink = expf(m - base), w = expf(s - base);
-            m = top;
-            l = fmaf(l, shrink, w);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = fmaf(acc[j], shrink, w * v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int d = j * GROUP + lane;
-            const float result = l == 0.f ? acc[j] * 0.f : acc[j] / l;
-            const long long to = (long long)(tok0 + r) * out_stride + (long long)h * head_dim + d;
-            if (d < head_dim) {
-                if (wide) reinterpret_cast<float*>(out)[to] = result;
-                else reinterpret_cast<__nv_bfloat16*>(out)[to] = __float2bfloat16_rn(result);
-            }
-        }
-    }
-}
 
 template <int HD, bool CAPPED>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -691,8 +628,9 @@ prompts_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, void* __
         for (int other = 0; other < shares; ++other) strange |= ld_cluster_u32(strange_s, other);
     }
     if (strange) {
-        rows_again(q, q_stride, out, out_stride, extras.wide, cache, table_row, head_at, h, head_dim, tok0, pos0, rows, window, scale, softcap, extras.sink,
-                   share * (THREADS / 32) + warp, shares * (THREADS / 32), lane);
+        for (int r = share * (THREADS / 32) + warp; r < rows; r += shares * (THREADS / 32))
+            row_again(q + (long long)(tok0 + r) * q_stride + (long long)h * head_dim, out, (long long)(tok0 + r) * out_stride + (long long)h * head_dim, extras.wide,
+                      cache, table_row, head_at, head_dim, pos0 + r, window, scale, softcap, extras.sink ? extras.sink + h : nullptr, lane);
     } else if (shares > 1) {
         // a part of the rows each, eight numbers a thread
         constexpr int PIECES = HD / 8;

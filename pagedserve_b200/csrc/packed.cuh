@@ -51,6 +51,68 @@ struct Pages {
     }
 };
 
+struct Cache {
+    const unsigned char* k_pool;
+    const unsigned char* v_pool;
+    long long page_stride;
+    Pages pages;
+};
+
+// One bfloat16 query against the keys that position p sees, in float32 from the codes, for kernels whose float16 operands do not hold them: lane l of the warp has
+// number 32 j + l of every group (heads of up to 128), key after key. `out` from `to` on: bfloat16, or float32 where `wide`; `sink`: null, or the head's. Slow: a key is
+// a chain of page, codes and score (about 0.4 us).
+template <typename T>
+__device__ __noinline__ void row_again(const T* q, void* out, long long to, int wide, const Cache cache, int table_row, long long head_at, int head_dim, int p,
+                                       int window, float scale, float softcap, const float* sink, int lane) {
+    const int groups = groups_of(head_dim), page_size = 1 << cache.pages.page_log2, shift = code_shift(lane & 7);
+    const int last = min(p, (cache.pages.bt_stride << cache.pages.page_log2) - 1);
+    float x[4], acc[4], m = -INFINITY, l = 0.f;
+    if (sink) {
+        m = *sink;
+        l = 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int d = j * GROUP + lane;
+        x[j] = d < head_dim ? to_float(q[d]) : 0.f;
+        acc[j] = 0.f;
+    }
+    for (int key = p < 0 ? 0 : first_visible_key(p, window); key <= last; ++key) {
+        const int page = cache.pages.of(table_row, key);
+        if (page < 0) continue;
+        const long long at = (long long)page * cache.page_stride + head_at;
+        const int row = key & (page_size - 1);
+        float s = 0.f, v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = 0.f;
+            if (j < groups) {
+                const int word = (row * 4 + (lane >> 3)) * groups + j, scale_at = page_size * groups * 4 + row * groups + j;
+                const uint32_t *k = reinterpret_cast<const uint32_t*>(cache.k_pool + at), *w = reinterpret_cast<const uint32_t*>(cache.v_pool + at);
+                const bool there = j * GROUP + lane < head_dim;                // (a number that is not there has no code)
+                if (there) s = fmaf(fmaf((float)(k[word] >> shift & 15u), step_of(k[scale_at]), low_of(k[scale_at])), x[j], s);
+                v[j] = fmaf((float)(w[word] >> shift & 15u), step_of(w[scale_at]), low_of(w[scale_at]));
+            }
+        }
+        s = warp_sum(s) * scale;
+        if (softcap > 0.f) s = softcap * tanhf(s / softcap);
+        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, shrink = expf(m - base), w = expf(s - base);
+        m = top;
+        l = fmaf(l, shrink, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(acc[j], shrink, w * v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int d = j * GROUP + lane;
+        const float result = l == 0.f ? acc[j] * 0.f : acc[j] / l;             // (no key at all: zero; a NaN stays one)
+        if (d < head_dim) {
+            if (wide) reinterpret_cast<float*>(out)[to + d] = result;
+            else reinterpret_cast<T*>(out)[to + d] = from_float<T>(result);
+        }
+    }
+}
+
 inline bool sizes_ok(int n_kv_heads, int head_dim, int page_size) {
     return n_kv_heads > 0 && head_dim > 0 && head_dim <= MAX_HEAD && page_size > 0 && page_size <= 64 && !(page_size & (page_size - 1));
 }

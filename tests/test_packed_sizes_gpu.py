@@ -98,6 +98,73 @@ def test_sinks_far_above_the_scores(dtype, shares, sink, window, softcap):
     agrees(prompts(ops, case, planes, q, new, heads, 0.125, **extras), found, limit)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1e-4, 1e-5, 1e-6, 3e-8, 1e-12])
+@pytest.mark.parametrize("what", ["a group of values", "a group of one value", "the first rows' values", "a channel", "a group of keys", "the last values"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 2, 128), (3, 1, 40), (20, 2, 96)])
+def test_small_numbers_of_single_tokens(dtype, size, what, heads, kv_heads, dim):
+    """As in prompts."""
+    ops, case, planes, q, positions, scale, found = beside_ordinary_ones(dtype, size, what, heads, kv_heads, dim, 300)
+    if what == "a channel":
+        # Single tokens form a group's part of the result as a sum of step * (code - 8) and one of low + 8 * step, both of the group's size whatever the number
+        # itself: their roundings, counted by a channel's own numbers in the limit, count by the largest channel's of the group here.
+        groups = torch.arange(dim) // 32
+        found = found[0], torch.stack([found[1][..., groups == g].amax(-1) for g in groups], -1), found[2]
+    some = [0, 1, 39, 150, 299]
+    found = [x[some] for x in found]
+    agrees(tokens(ops, case, planes, q[some], positions[some].tolist(), heads, scale), found, limit_of(found, scale, dtype, dim))
+
+
+def heavy_key(dtype, heads, kv_heads, dim, length, place, gap, seed):
+    """Queries that one key, at ``place``, answers with a score about ``gap`` above all others'."""
+    g = torch.Generator().manual_seed(seed)
+    case = PackedCase([length], kv_heads, dim, 16, dtype, seed=seed, mean=0.0)
+    along = torch.randn(kv_heads, dim, generator=g)
+    along /= along.norm(dim=1, keepdim=True)
+    case.k = (case.k.float() * 0.25 - (case.k.float() * 0.25 * along).sum(-1, keepdim=True) * along).to(dtype)
+    case.k[place] = (8 * along).to(dtype)
+    q = (along.repeat_interleave(heads // kv_heads, 0) * (gap * dim ** 0.5 / 8))[None] + 0.05 * torch.randn(6, heads, dim, generator=g)
+    return case, q.flatten(1).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 128), (20, 2, 32), (2, 1, 96)])
+@pytest.mark.parametrize("shrink", [10, 16, 18, 20, 24, 30, 60])
+@pytest.mark.parametrize("place", [0, 150, 690])
+def test_the_key_that_carries_the_weight_has_small_values(dtype, heads, kv_heads, dim, shrink, place):
+    """The result is that key's values, however much larger those of the keys are that have no weight."""
+    ops, length = ops_for(dtype), 700
+    case, q = heavy_key(dtype, heads, kv_heads, dim, length, place, 60.0, dim)
+    case.v[place] = (case.v[place].float() * 2.0 ** -shrink).to(dtype)
+    if shrink == 20:
+        case.v[place, :, :16] *= 64.0                                     # (a step and a low that are not alike)
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    positions, scale = torch.arange(length - 6, length), dim ** -0.5
+    found = attention(q.double().view(6, heads, dim), k, v, positions, scale)
+    limit = limit_of(found, scale, dtype, dim)
+    for shares in (0, 1, 8):
+        agrees(tokens(ops, case, planes, q, positions.tolist(), heads, scale, shares=shares), found, limit)
+    agrees(prompts(ops, case, planes, q, 6, heads, scale), found, limit)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("gap", [6.0, 10.0, 12.0, 16.0, 20.0])
+def test_the_key_that_carries_the_weight_has_no_values(dtype, heads, kv_heads, dim, gap):
+    """A key whose values are zeros takes the weight: the others' small weights make the result."""
+    ops, length = ops_for(dtype), 300
+    case, q = heavy_key(dtype, heads, kv_heads, dim, length, 3, gap, dim)
+    case.v[3] = 0
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    positions, scale = torch.arange(length - 6, length), dim ** -0.5
+    found = attention(q.double().view(6, heads, dim), k, v, positions, scale)
+    limit = limit_of(found, scale, dtype, dim)
+    agrees(tokens(ops, case, planes, q, positions.tolist(), heads, scale), found, limit)
+    agrees(prompts(ops, case, planes, q, 6, heads, scale), found, limit)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim", [(12, 12, 64), (8, 2, 128)])
 def test_results_repeat_bit_by_bit(heads, kv_heads, dim):
     ops, length, new = ops_for(BF16), 900, 300
