@@ -2386,7 +2386,7 @@ class Ops:
                                            _ptr(results.top_logprobs), _ptr(results.top_ids), _ptr(status), _stream()), what)
         return results
 
-    FUSED_HEAD_VOCABULARY, FUSED_HEAD_MOST, SAMPLED = 8192, 4096, 2048
+    FUSED_HEAD_VOCABULARY, FUSED_HEAD_MOST, SAMPLED, HEAD_LIST = 8192, 4096, 2048, 2048
 
     def fused_head_ok(self, x, table, top=0):
         """Whether the log probabilities of these rows are read inside the head's product: bfloat16, a large vocabulary, and so many rows that the
@@ -2399,6 +2399,13 @@ class Ops:
         least = 16 if not top else 48 if V > 40000 else 128
         return self.dtype == torch.bfloat16 and rows >= least and V >= self.FUSED_HEAD_VOCABULARY and self.tc_ok(x, table)
 
+    @classmethod
+    def sample_every(cls, V, top):
+        """Which tokens (every how many) bound the alternatives of a row: about ``SAMPLED`` of the vocabulary, more where what lies beyond the bound might not fit the
+        row's list. Of tokens in no order by their logits that is the sum of ``top`` waits of ``every`` tokens on average, and longer than ``every`` (top + 6 sqrt(top) +
+        12) in fewer than one row of a million (Chernoff's bound). A row whose list overflows is formed again by one CTA, which reads the whole table."""
+        return min(-(-V // cls.SAMPLED), int(cls.HEAD_LIST / (top + 6 * top ** 0.5 + 12)))
+
     def _fused_head(self, x, table, targets, top, status, results):
         (rows, K), V, device = x.shape, table.shape[0], x.device
         library = self._packed_library()
@@ -2407,14 +2414,14 @@ class Ops:
         sample = entries = count = limit = limit_index = None
         every, n = 1, V
         if top:
-            every = -(-V // self.SAMPLED)
+            every = self.sample_every(V, top)
             n = -(-V // every)
             sample = self.empty((rows, -(-n // 4) * 4), torch.float32, device)
             if rows > 1024:                              # (2,047 x 2,011 x 768: 10 us in tiles 256 wide, 17 in 128)
                 self.linear_tc(x, table[::every], None, sample[:, :n], bn=256)
             else:
                 self.linear(x, table[::every], None, sample[:, :n])
-            entries = self.empty((rows, 2048), torch.int64, device)
+            entries = self.empty((rows, self.HEAD_LIST), torch.int64, device)
             count, limit_index = self.empty((rows,), torch.int32, device), self.empty((rows,), torch.int32, device)
             limit = self.empty((rows,), torch.float32, device)
         self.launches += 3 if top else 2
