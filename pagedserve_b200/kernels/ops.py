@@ -2451,7 +2451,10 @@ class Ops:
         if self.fused_head_ok(x, table, top):
             for start in range(0, rows, self.FUSED_HEAD_MOST):
                 part = slice(start, min(rows, start + self.FUSED_HEAD_MOST))
+                mark = self.arena.mark() if self.arena is not None else None
                 self._fused_head(x[part], table, targets[part], top, status, TokenLogprobs(*(result[part] for result in results)))
+                if mark is not None:
+                    self.arena.release(mark)                  # (a piece's scratch, 24 KB a row, is the next one's)
             return results
         at_once = max(128, self.LOGITS_AT_ONCE // V // 128 * 128)
         # (rows of whole 16-byte pieces: the product stores them by TMA)

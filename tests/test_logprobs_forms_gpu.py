@@ -92,6 +92,27 @@ def test_large_vocabularies(rows, V, top):
     check(found, x.double() @ table.double().t(), targets, top)
 
 
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("most", [128, 200])
+def test_pieces_of_many_rows(top, most):
+    """Rows in pieces of FUSED_HEAD_MOST, the last one short, from a step's arena and without one."""
+    from pagedserve_b200.kernels.ops import StepArena
+
+    ops = ops_for(BF16)
+    x, table, targets = on_a_grid(517, 96, 9000, 3)
+    x, table = x.to(BF16), table.to(BF16)
+    whole = ops.head_logprobs(x, table, targets, top)
+    logits = x.double() @ table.double().t()
+    check(whole, logits, targets, top)
+    ops.FUSED_HEAD_MOST = most
+    check(ops.head_logprobs(x, table, targets, top), logits, targets, top)
+    ops.arena = StepArena()
+    ops.empty((1000,), torch.float32, x.device)
+    before = ops.arena.mark()
+    check(ops.head_logprobs(x, table, targets, top), logits, targets, top)
+    assert ops.arena.mark() == before                                      # (a piece's scratch is the next one's)
+
+
 @pytest.mark.parametrize("top", [0, 4])
 def test_a_captured_fused_head(top):
     """Captured on a side stream and replayed with other rows."""
