@@ -1353,6 +1353,11 @@ class Ops:
             window or 0, scale, float(softcap or 0.0), _ptr(sink), shares, together, self.code, _stream()), what)
         return out
 
+    @staticmethod
+    def unpacked_span(max_kv_len):
+        """Positions of an item whose rows are unpacked for prompts in float32: whole pages of 64."""
+        return -(-int(max_kv_len) // 64) * 64
+
     UNPACKED_BYTES = 512 << 20        # most scratch that prompts take whose rows are unpacked first (but one item's rows always)
 
     def _counting(self, count, device):
@@ -1402,7 +1407,8 @@ class Ops:
             return out
         # float32: the rows as pages of the compute type, some items at a time, and the kernels for those.
         page = 64
-        span = min(-(-int(max_kv_len) // page) * page, -(-block_table.shape[1] * page_size // page) * page)
+        # (room for every position that a context may have, whether the table has a page for it or not: the kernels look no position up that has no place here)
+        span = self.unpacked_span(max_kv_len)
         item_bytes = span * 2 * n_kv_heads * head_dim * self.dtype.itemsize
         at_once = max(1, min(n_items, self.UNPACKED_BYTES // item_bytes))
         scratch = self.empty((at_once * (span // page), 2, n_kv_heads, page, head_dim), self.dtype, device)

@@ -177,3 +177,19 @@ def test_results_repeat_bit_by_bit(heads, kv_heads, dim):
         at = list(range(length - 8, length))
         one, two = (tokens(ops, case, planes, q[:8], at, heads, 0.125, shares=shares) for _ in range(2))
         assert torch.equal(one, two)
+
+
+def test_contexts_longer_than_their_table_in_float32():
+    """What has no place in the table is a key of zeros, as a key without a page is: the kernels stay inside the unpacked rows."""
+    ops, heads, dim, page, width = ops_for(F32), 2, 64, 16, 5
+    case = PackedCase([width * page, width * page], heads, dim, page, F32, seed=3)
+    _, planes = on_device(case)
+    lengths, new = [600, 333], [200, 333]
+    q = torch.randn(sum(new), heads * dim, generator=torch.Generator().manual_seed(3))
+    out = torch.full((sum(new), heads * dim), 7.0, device=DEV)
+    ops.packed_attention_prompts(q.to(DEV), out, *planes, ints([0, 200, 533]), ints(lengths), case.table.to(DEV), ints([0, 1]), 0, 2, 4 + 6, max(lengths), heads, heads, dim,
+                                 page, None, 0.125)
+    for item, rows in enumerate((slice(0, 200), slice(200, 533))):
+        k, v = (torch.cat([case.context(item, x), torch.zeros(lengths[item] - width * page, heads, dim, dtype=torch.float64)]) for x in case.held())
+        found = attention(q[rows].double().view(-1, heads, dim), k, v, torch.arange(lengths[item] - new[item], lengths[item]), 0.125)
+        agrees(out[rows].cpu().double().view(-1, heads, dim), found, limit_of(found, 0.125, F32, dim))
