@@ -32,6 +32,18 @@ def kv_cache_budget(free_memory: int, total_memory: int,
     return budget
 
 
+def unpacking_reserve(needs, max_model_len: int, max_num_seqs: int) -> int:
+    """Bytes that prompts in float32 over a cache of 4 bits may take besides: their rows unpacked, some requests' at a time (at most
+    ``Ops.UNPACKED_BYTES``, but one request's always), in scratch of sizes that are powers of two and are kept, together less than twice the largest."""
+    from pagedserve_b200.kernels.ops import Ops
+
+    most = 0
+    for need in needs:
+        one = Ops.unpacked_span(max_model_len) * 2 * need.n_kv_heads * need.head_dim * 4
+        most = max(most, min(max(Ops.UNPACKED_BYTES, one), one * max_num_seqs))
+    return 2 * Ops.unpacked_bytes(most) if most else 0
+
+
 def pages_for_budget(budget_bytes: int, bytes_per_page: int, max_num_seqs: int, max_model_len: int,
                      block_size: int) -> int:
     """Pages of ``bytes_per_page`` within ``budget_bytes``, no more than the live requests can hold."""

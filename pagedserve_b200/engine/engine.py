@@ -11,7 +11,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 
 import torch
 
-from pagedserve_b200.cache.budget import MIB, kv_cache_budget, pages_for_budget
+from pagedserve_b200.cache.budget import MIB, kv_cache_budget, pages_for_budget, unpacking_reserve
 from pagedserve_b200.cache.manager import CacheManager
 from pagedserve_b200.config.engine_config import UNBOUNDED_MODEL_LEN, EngineConfig
 from pagedserve_b200.config.registry import ConfigError, ModelConfig, load_config_dict, resolve_architecture
@@ -105,7 +105,10 @@ class Engine:
         else:
             # reference: main.py:186-200 (budget from the device's free and total memory)
             free, total = torch.cuda.mem_get_info(self.device)
-            budget = kv_cache_budget(free, total, cfg.kv_cache_memory_utilization, cfg.kv_cache_safety_mb * MIB)
+            kept = cfg.kv_cache_safety_mb * MIB
+            if packed and self.dtype == torch.float32:
+                kept += unpacking_reserve(by_need, self.spec.max_model_len, cfg.max_num_seqs)
+            budget = kv_cache_budget(free, total, cfg.kv_cache_memory_utilization, kept)
             num_pages = pages_for_budget(budget, bytes_per_page, cfg.max_num_seqs, self.spec.max_model_len,
                                          cfg.block_size)
         return CacheManager(kv_needs, state_needs, cfg.block_size, int(num_pages), cfg.max_num_seqs,

@@ -1358,6 +1358,12 @@ class Ops:
         """Positions of an item whose rows are unpacked for prompts in float32: whole pages of 64."""
         return -(-int(max_kv_len) // 64) * 64
 
+    @staticmethod
+    def unpacked_bytes(needed):
+        """What is asked for where rows of ``needed`` bytes are unpacked: a power of two. A step's arena gives nothing back, and as a context grows, every portion of a prompt
+        needs a little more than the last one did: chunk behind chunk, 13 GB for one prompt of 32,768 positions (25 heads of 64, portions of 512)."""
+        return 1 << (int(needed) - 1).bit_length()
+
     UNPACKED_BYTES = 512 << 20        # most scratch that prompts take whose rows are unpacked first (but one item's rows always)
 
     def _counting(self, count, device):
@@ -1411,7 +1417,8 @@ class Ops:
         span = self.unpacked_span(max_kv_len)
         item_bytes = span * 2 * n_kv_heads * head_dim * self.dtype.itemsize
         at_once = max(1, min(n_items, self.UNPACKED_BYTES // item_bytes))
-        scratch = self.empty((at_once * (span // page), 2, n_kv_heads, page, head_dim), self.dtype, device)
+        scratch = self.empty((self.unpacked_bytes(at_once * item_bytes) // self.dtype.itemsize,), self.dtype, device)
+        scratch = scratch[:at_once * item_bytes // self.dtype.itemsize].view(at_once * (span // page), 2, n_kv_heads, page, head_dim)
         counting = self._counting(at_once * (span // page), device)
         table = counting[:at_once * (span // page)].view(at_once, span // page)
         for start in range(first_item, first_item + n_items, at_once):

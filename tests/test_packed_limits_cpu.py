@@ -2,6 +2,8 @@
 
 import math
 
+import pytest
+
 
 def test_what_lies_beyond_a_sample_fits_the_lists():
     """Whatever the vocabulary and the alternatives: fewer than one row of a million overflows, and the sample has enough tokens."""
@@ -25,3 +27,38 @@ def test_unpacked_rows_have_a_place_for_every_position():
     for longest in (1, 63, 64, 65, 100, 1000, 4097, 32768):
         span = Ops.unpacked_span(longest)
         assert span % 64 == 0 and (longest - 1) // 64 < span // 64 and span < longest + 64
+
+
+@pytest.mark.parametrize("kv_heads,dim,longest,portion", [(25, 64, 32768, 512), (12, 64, 1024, 128), (8, 128, 131072, 4096)])
+def test_unpacked_rows_of_a_growing_context(kv_heads, dim, longest, portion):
+    """A step's arena keeps what it was ever asked for: a prompt that runs in portions must not ask for a little more with each of them."""
+    import torch
+
+    from pagedserve_b200.cache.budget import unpacking_reserve
+    from pagedserve_b200.cache.manager import KVNeed
+    from pagedserve_b200.kernels.ops import Ops, StepArena
+
+    def grown(asked):
+        arena = StepArena()
+        for end in range(portion, longest + 1, portion):
+            arena.reset()
+            arena.empty((asked(Ops.unpacked_span(end) * 2 * kv_heads * dim * 4) // 4,), torch.float32, torch.device("meta"))
+        return sum(chunk.numel() - StepArena.ALIGN for chunk in arena.chunks)
+
+    largest = longest * 2 * kv_heads * dim * 4
+    reserve = unpacking_reserve([KVNeed(kv_heads, dim)], longest, 64)
+    assert grown(Ops.unpacked_bytes) <= max(reserve, StepArena.CHUNK_BYTES)
+    assert largest <= reserve <= 4 * max(largest, Ops.UNPACKED_BYTES)
+    if largest > 4 * StepArena.CHUNK_BYTES:
+        assert grown(lambda needed: needed) > 4 * reserve                  # (as it would be otherwise)
+
+
+def test_what_is_kept_for_unpacked_rows():
+    from pagedserve_b200.cache.budget import unpacking_reserve
+    from pagedserve_b200.cache.manager import KVNeed
+
+    assert unpacking_reserve([], 1024, 8) == 0
+    assert unpacking_reserve([KVNeed(12, 64)], 1024, 1) == 2 * (1 << 23)                   # 6 MB of one request
+    assert unpacking_reserve([KVNeed(12, 64), KVNeed(25, 64)], 1024, 8) == 2 * (1 << 27)   # 8 requests of 13 MB
+    assert unpacking_reserve([KVNeed(25, 64)], 1024, 1000) == 2 * (1 << 29)
+    assert unpacking_reserve([KVNeed(32, 128)], 10 ** 5, 8) == 2 * (1 << 32)               # one request's rows, whatever they need
