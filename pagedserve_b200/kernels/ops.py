@@ -1192,6 +1192,8 @@ class Ops:
         """Checks what the kernels over a packed cache (csrc/packed.cuh) share; the pages of the pools."""
         if not (0 < head_dim <= PACKED_MAX_HEAD) or page_size not in (1, 2, 4, 8, 16, 32, 64):
             raise KernelError(f"{what}: head sizes up to {PACKED_MAX_HEAD}, pages of a power of two up to 64 tokens")
+        if block_table.shape[-1] * page_size > MOST_COUNT:            # (a kernel counts positions in 32 bits)
+            raise KernelError(f"{what}: block_table rows of up to {MOST_COUNT} positions")
         slab = packed_slab_bytes(page_size, head_dim)
         shape, strides, device = k_pool.shape, (page_stride, slab, 1), k_pool.get_device()
         if not (len(shape) == 3 and shape[1] == n_kv_heads and shape[2] == slab and k_pool.stride() == strides and v_pool.shape == shape

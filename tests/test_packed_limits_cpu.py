@@ -62,3 +62,19 @@ def test_what_is_kept_for_unpacked_rows():
     assert unpacking_reserve([KVNeed(12, 64), KVNeed(25, 64)], 1024, 8) == 2 * (1 << 27)   # 8 requests of 13 MB
     assert unpacking_reserve([KVNeed(25, 64)], 1024, 1000) == 2 * (1 << 29)
     assert unpacking_reserve([KVNeed(32, 128)], 10 ** 5, 8) == 2 * (1 << 32)               # one request's rows, whatever they need
+
+
+def test_tables_of_more_positions_than_are_counted_are_refused():
+    """(single tokens over a table of 2^31 positions saw none of them)"""
+    import torch
+
+    from pagedserve_b200.kernels.ops import KernelError, Ops, packed_slab_bytes
+
+    ops, page, dim = Ops(torch.bfloat16), 64, 64
+    slab = packed_slab_bytes(page, dim)
+    pool = torch.empty((2, 2, 1, slab), dtype=torch.uint8)
+    ask = lambda width: ops._packed_pools("packed_attention_tokens", pool[:, 0], pool[:, 1], 2 * slab, 1, dim, page, torch.empty((1, width), dtype=torch.int32, device="meta"))
+    with pytest.raises(KernelError, match="positions"):
+        ask(2 ** 25)
+    with pytest.raises(KernelError, match="CUDA device"):
+        ask(2 ** 25 - 2 ** 10)
