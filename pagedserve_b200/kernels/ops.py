@@ -1386,11 +1386,14 @@ class Ops:
         blocks they make up, ``max_kv_len`` >= their contexts.  ``q`` / ``out`` are the step's flat token arrays; item i's tokens are rows
         ``q_start[i] .. q_start[i + 1]``, the last ones of ``kv_len[i]``, its pages row ``item_row[i]`` of ``block_table``.  A key without a page is
         not seen in bfloat16 and is one of zeros in float32, as it is over pages of the compute type.  ``shares`` (bfloat16): CTAs for the keys of 256
-        queries, 1, 2, 4 or 8 (0: by the counts).  Otherwise as :meth:`prefill_attention`."""
+        queries, 1, 2, 4 or 8 (0: by the counts).  ``out`` is not ``q``: rows that float16 does not hold are formed again, from their queries, behind the
+        others' results.  Otherwise as :meth:`prefill_attention`."""
         what = "packed_attention_prompts"
         n_pages = self._packed_pools(what, k_pool, v_pool, page_stride, n_kv_heads, head_dim, page_size, block_table)
         device = k_pool.get_device()
         self._packed_queries(what, q, out, n_heads, n_kv_heads, head_dim, scale, softcap, sink, device)
+        if q.data_ptr() == out.data_ptr() and q.numel():
+            raise KernelError(f"{what}: the results cannot take the queries' place")
         if first_item < 0 or n_items < 0:
             raise KernelError(f"{what}: items below 0")
         self._indices(what, first_item + n_items, device, kv_len=kv_len, item_row=item_row)

@@ -193,3 +193,19 @@ def test_contexts_longer_than_their_table_in_float32():
         k, v = (torch.cat([case.context(item, x), torch.zeros(lengths[item] - width * page, heads, dim, dtype=torch.float64)]) for x in case.held())
         found = attention(q[rows].double().view(-1, heads, dim), k, v, torch.arange(lengths[item] - new[item], lengths[item]), 0.125)
         agrees(out[rows].cpu().double().view(-1, heads, dim), found, limit_of(found, 0.125, F32, dim))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_results_in_the_queries_place(dtype):
+    """Single tokens read a head's query before its result is written, done again or not; prompts refuse it."""
+    from pagedserve_b200.kernels.ops import KernelError
+
+    ops, case, planes, q, positions, scale, found = beside_ordinary_ones(dtype, 1e-12, "a group of keys", 4, 2, 64, 300)
+    limit, some = limit_of(found, scale, dtype, 64), [0, 17, 299]
+    rows = q[some].to(DEV)
+    ops.packed_attention_tokens(rows, rows, *planes, ints([0] * 3), ints(positions[some].tolist()), case.table.to(DEV), 4, 2, 64, 16, None, scale, 700)
+    agrees(rows.cpu().double().view(3, 4, 64), [x[some] for x in found], limit[some])
+    rows = q.to(DEV)
+    with pytest.raises(KernelError, match="place"):
+        ops.packed_attention_prompts(rows, rows, *planes, ints([0, 300]), ints([700]), case.table.to(DEV), ints([0]), 0, 1, 5, 700, 4, 2, 64, 16, None, scale)
+    assert torch.equal(rows.cpu(), q)
