@@ -14,7 +14,7 @@
 // thread-block cluster and merge through shared memory, in the order of the shares.
 //
 // What bounds it: instructions, two to four for every code of a key and of a value (5 tokens of up to 777 keys, the last 512 seen, 16
-// heads of 64, capped scores, a sink: 8.3 us for 3.2 MB; 64 tokens of 1,024 keys, 12 heads of 64, 33), and for few
+// heads of 64, capped scores, a sink: 7.6 us for 3.2 MB; 64 tokens of 1,024 keys, 12 heads of 64, 34), and for few
 // tokens the chain of page, keys, weights and values of a tile: the values of 16 keys (2 groups a head) are on their way while the scores are formed (one
 // token of 32,768 keys 56 us; with four at a time, asked for when they are due, 101).
 #include "packed.cuh"

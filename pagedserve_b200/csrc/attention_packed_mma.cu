@@ -20,11 +20,12 @@
 // A CTA has a token, a key head (8 or 16 of its query heads) and a share of the keys; a warp takes tiles of 16 keys, which it brings to shared
 // memory itself (cp.async, a ring of its own, no barrier). Shares are a cluster and merge through shared memory.
 //
-// What bounds it: instructions, not bytes (the same time with one page that every token shares). A tile of 16 keys is about 600 instructions a warp at
-// 128 numbers a head and 8 queries, half of them masks, shifts and sums on the ALU pipe, which issues every other clock (44 - 51 % busy; a warp's own chain
-// of scores, weights and products leaves the rest idle); its 32 mma.sync are not felt. 64 tokens of 4,099 keys, 32 heads on 8 of 128: 102 us, 2.3 TB/s;
-// 64 x 1,024, 12 heads of 64: 28 us; one token of 32,768: 26 us, 12 heads by 8 shares of 8 warps on 148 SMs. A page's number is asked for a tile before it
-// is used and not compared until then, or its latency stands in the loop (110 us; one token 46, so 36 with 4 warps).
+// What bounds it: instructions, not bytes (the same time with one page that every token shares). A tile of 16 keys is about 640 instructions a warp at
+// 128 numbers a head and 8 queries, half of them masks, shifts and sums on the ALU pipe, which issues every other clock (59 % of its slots on average, 73 % on the
+// busiest SM; 63 % of all issue slots: a warp's own chain of scores, weights and products leaves the rest idle); its 32 mma.sync are not felt. 64 tokens of 4,099
+// keys, 32 heads on 8 of 128: 103 us, 2.3 TB/s; 64 x 1,024, 12 heads of 64: 29 us; one token of 32,768: 26 us, 12 heads by 8 shares of 8 warps on 148 SMs. A
+// page's number is asked for a tile before it is used and not compared until then, or its latency stands in the loop (110 us; one token 46, so 36 with 4 warps). A token
+// that is done again takes 60 us for 129 keys and 480 for 1,024.
 #include "packed.cuh"
 
 namespace ps {

@@ -21,10 +21,12 @@
 // Few blocks of many keys: a cluster's CTAs share the key tiles out, leave O, bases and sums in shared memory and join a part of the rows each; a block of
 // few keys takes fewer of them, and the others end at once.
 //
-// What bounds it: per 128 keys and 256 queries the rows' instructions (about 2,500 clocks, 2,048 of them exponentials) at head size 64, the makers' (about
-// 2,500, keys and values) at 128; and about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
-// codes) and the first passes through everything. Two prompts of 1,024 (12 heads of 64) 25.6 us; three portions of 683 and fewer queries
-// behind up to 8,192 keys (16 heads on 4 of 128) 170 us, 0.62 PFLOP/s. The way there at those two: an MMA issued behind `lane == 0`, or predicated, takes 70 to 97
+// What bounds it: per 128 keys and 256 queries the rows' instructions are about 2,500 clocks, 2,048 of them exponentials, and at head size 128 the makers' about 2,500
+// (keys and values), the products' 2,050; a tile takes about 5,000 there, with 54 % of the issue slots and 42 % of the tensor pipe used: the roles wait for one another,
+// and which of the waits it is has not been measured. Then about 12,000 clocks from a CTA's start to its first weights, four dependent reads (lengths, row, page,
+// codes) and the first passes through everything. Two prompts of 1,024 (12 heads of 64) 25.1 us; three portions of 683 and fewer queries
+// behind up to 8,192 keys (16 heads on 4 of 128) 170 us, 0.62 PFLOP/s. Rows that are formed again take a warp 0.4 us a key: 250 us for a prompt of 129, 7.5 ms where
+// all blocks of two prompts of 1,024 do. The way there at those two: an MMA issued behind `lane == 0`, or predicated, takes 70 to 97
 // clocks, behind elect.sync 45 (190 -> 182 us at head size 128, one query tile 68 -> 54); the queries by the rows' warps, which wait anyway, instead of the
 // makers (26.8 -> 25.6, 182 -> 170). Two threads a row, 32 scores each, were slower (30 us, 190: a meeting of the two each half, and 80 registers a thread), and so were six
 // makers with halves of rows (27, 211: the groups' numbers twice, a page for each).

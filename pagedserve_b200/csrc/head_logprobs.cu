@@ -5,7 +5,8 @@
 //             to its 256 rows and walks a strip of the vocabulary, so that the sums of a row stay in the registers of its four threads (each takes
 //             every fourth 32 tokens of a tile); a strip leaves m, S and W of its part of a row.  A warp reads 32 tokens of its rows in about
 //             2,300 clocks, most of them waits for results, so that with two threads a row the reading was longer than the product.
-// sample      for the most likely tokens, the logits of every s-th token (about 2,048 of them) are formed first, by the ordinary product: the `top`-th
+// sample      for the most likely tokens, the logits of every s-th token (about 2,048 of them, more for vocabularies and lists beyond 50,257 and 32: what lies beyond
+//             the bound is to fit a row's list) are formed first, by the ordinary product: the `top`-th
 //             largest of them is a bound that the row's `top` largest reach, less 2^-16 of itself, since another product may add in another order.
 //             The product sends what lies beyond it (about 25 * top of 50,257) to a list of its row: a number larger than the bound, or equal to it
 //             up to the sampled token that set it, so that whatever is not in the list comes behind all that is.  A thread holds up to 16 of them in
@@ -14,9 +15,11 @@
 // join        a CTA a row adds the strips' sums up, ranks the list, and writes the results.  A row whose list did not hold all (an order of tokens that
 //             fools the sample), or fewer than `top`, has its logits formed again there, token by token.
 //
-// What bounds it, 2,047 rows of 768 on 50,257 tokens (158 GFLOP, 96 us at a cuBLAS product's measured rate): without alternatives the tensor pipe, 94 us
-// (112 with the MMAs issued behind `lane == 0` instead of elect.sync); with 5 of them 157, of which the sample's product and ranking are about 25, the join 13,
-// and numbers on their way to the lists 10; with 20 183. Up to about 256 rows (42 us; without alternatives 21) the table's 77 MB and four kernels one behind another.
+// What bounds it, 2,047 rows of 768 on 50,257 tokens (158 GFLOP, 96 us at a cuBLAS product's measured rate): without alternatives the tensor pipe, 91 % of the time
+// active, 94 us (112 with the MMAs issued behind `lane == 0` instead of elect.sync); with 5 of them 157, with 20 183. One by one, in front of cold caches: the product
+// 100 without alternatives and 127 with 5 (five stages for six, tensor memory read twice, numbers on their way to the lists: the tensor pipe 68 % active), the sample's
+// product 18 and ranking 16, the join 17 (without alternatives 11). Up to about 256 rows (42 us; without alternatives 21) the table's 77 MB and four kernels one
+// behind another.
 #include <cuda.h>
 
 #include "logprobs.cuh"
@@ -159,7 +162,7 @@ sample_kernel(const float* __restrict__ logits, long long ld, int n, int every, 
     const List list = {entry_s, kept_s, &count_s, &limit_s, group_s, &bound_s};
     if (tid == 0) { count_s = 0; limit_s = 0; }
     __syncthreads();
-    for (int chunk = 0; chunk < n; chunk += CHUNK) {                // (once, as the engine takes it)
+    for (int chunk = 0; chunk < n; chunk += CHUNK) {
         float x[PER], big = -INFINITY;
 #pragma unroll
         for (int u = 0; u < PER; ++u) {

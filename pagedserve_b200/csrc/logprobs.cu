@@ -3,11 +3,11 @@
 // of equal logits the lower index first.  A token of -1 is none: its log probability is 0.  One outside the vocabulary sets *status and gets NaN.
 // A NaN or +infinity among the logits makes a row's numbers NaN; -infinity is a token of probability 0.  NaN comes behind all others in the order.
 //
-// One pass over a row, which is all its traffic: a thread has 8 numbers of a chunk of 2,048, two pieces of 16 bytes, the next two on their way.  m, S and W are kept by
+// One pass over a row, which is all its traffic: a thread has 8 numbers of a chunk (2,048; 4,096 in CTAs of 512 threads), two pieces of 16 bytes, the next two on their way.  m, S and W are kept by
 // thread, W moved to a new maximum m' by W' = e^(m - m') (W + (m - m') S).  Sums are float32, of about 200 numbers a thread and
 // then of the threads by halving exchanges.
 //
-// The largest: 64 groups of 32 numbers each give their largest; the `top`-th of those is a bound that at least `top` numbers of the first chunk
+// The largest: 64 groups of a chunk's numbers (32 each; 64 in CTAs of 512 threads) give their largest; the `top`-th of those is a bound that at least `top` numbers of the first chunk
 // reach, and hardly more than twice as many do.  These go to a list, which is ranked (each entry counts those in front of it).  From then
 // on only numbers beyond the list's last join it, about top * (chunk size) / (numbers so far) a chunk, without a barrier; the list is looked at every four chunks and
 // ranked when it has grown by RANK_AT entries (a look at every chunk cost 60 us of 164 with 2,047 rows and 5 alternatives).  Where more joined than it

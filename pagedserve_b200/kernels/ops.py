@@ -1323,7 +1323,8 @@ class Ops:
             if not shares:
                 # Shares pay while the GPU has SMs without a CTA, from 128 keys each on, and beyond that (to 8 CTAs an SM) only where a share is
                 # long against their merge. Measured in us at 1, 2, 4, 8 shares: 8 x 1,024 keys (12 heads of 64) 11.5, 9.3, 9.6, 13.1;
-                # 1 x 32,768 244, 126, 66, 36; 64 x 1,024 28.2, 31.0, 43.7, 73.2; 64 x 4,099 (32 heads on 8 of 128) 120, 102, 107, 130.
+                # 1 x 32,768 244, 126, 66, 36; 64 x 1,024 28.2, 31.0, 43.7, 73.2; 64 x 4,099 (32 heads on 8 of 128) 120, 102, 107, 130. A captured decode step
+                # says the longest context of the model, whatever its tokens': with 32,768 of them 8 tokens of 12 heads get 8 shares.
                 ctas, shares = T * n_kv_heads * -(-n_heads // n_kv_heads // 16), 1
                 while shares < 8 and (ctas * shares * 2 <= 592 and shares * 2 <= keys // 128
                                       or ctas * shares * 2 <= 1184 and shares * 2 <= keys // 1024):
@@ -1440,7 +1441,9 @@ class Ops:
         each on.  Blocks of items alike in length are counted.
 
         us without / with: 128 queries behind 3,872 keys, 12 heads of 64, 49.1 / 18.2; 256 behind 744 22.8 / 16.8; a prompt of 2,048 36.7 / 32.8; two of
-        1,024 26.2 / 25.9; one of 1,024 with 25 heads, 150 CTAs with them, 22.4 / 28.0."""
+        1,024 26.2 / 25.9; one of 1,024 with 25 heads, 150 CTAs with them, 22.4 / 28.0.  Those are calls for these items alone: a step that the engine pads to a shape
+        that comes back brings its entries to a multiple of four, and the empty ones are counted like others. 128 queries behind 4,000 keys get 2 shares of 8 there, a
+        prompt of 2,048 one of 2."""
         shares, most = 1, -(-longest // 128) + 1
         if n_heads * blocks > 148:
             return shares, most
@@ -2411,8 +2414,9 @@ class Ops:
         logits' way to memory and back takes longer than what stands around that product.
 
         Inside / formed first, us: without alternatives 8 rows of 768 on 50,257 tokens 21.8 / 20.6, 16 22.9 / 26.1, 64 23.0 / 44.4; of 1,024 on 32,000 at 16
-        rows 21.2 / 24.5; of 768 on 9,000 11.4 / 12.2. With 5, whose sample and list are four kernels more: on 50,257 at 40 rows 36.3 / 34.5, 48 35.9 / 46.2,
-        96 39.1 / 43.7; on 32,000 at 33 rows 32.1 / 26.4, 64 32.3 / 42.0, 96 36.9 / 33.5, 128 36.7 / 37.1; on 9,000 at 128 27.4 / 27.0."""
+        rows 21.2 / 24.5; of 768 on 9,000 11.4 / 12.2. With 5, whose sample's product and ranking are two kernels more: on 50,257 at 40 rows 36.3 / 34.5, 48 35.9 / 46.2,
+        96 39.1 / 43.7; on 32,000 at 33 rows 32.1 / 26.4, 64 32.3 / 42.0, 96 36.9 / 33.5, 128 36.7 / 37.1; on 9,000 at 128 27.4 / 27.0.  (The rule leaves 64 rows on 32,000 out, whose
+        product takes longer than that of 96; between 32,000 and 50,257 nothing was measured.)"""
         rows, V = x.shape[0], table.shape[0]
         least = 16 if not top else 48 if V > 40000 else 128
         return self.dtype == torch.bfloat16 and rows >= least and V >= self.FUSED_HEAD_VOCABULARY and self.tc_ok(x, table)
