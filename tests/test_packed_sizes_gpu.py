@@ -209,3 +209,66 @@ def test_results_in_the_queries_place(dtype):
     with pytest.raises(KernelError, match="place"):
         ops.packed_attention_prompts(rows, rows, *planes, ints([0, 300]), ints([700]), case.table.to(DEV), ints([0]), 0, 1, 5, 700, 4, 2, 64, 16, None, scale)
     assert torch.equal(rows.cpu(), q)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (20, 2, 33, 1), (3, 3, 128, 64), (6, 1, 20, 4)])
+@pytest.mark.parametrize("window,softcap,with_sink", [(None, None, True), (70, 5.0, False), (-128, None, True)])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("shares", [1, 8])
+def test_rows_that_are_formed_again(heads, kv_heads, dim, page, window, softcap, with_sink, out_dtype, shares):
+    """In float32 from the codes, under masks, caps and sinks, in rows of a wider buffer, with pages that are missing, beside rows that are not formed again."""
+    ops, lengths, new = ops_for(BF16), [300, 200, 1], [150, 200, 1]
+    case = PackedCase(lengths, kv_heads, dim, page, BF16, seed=dim, width=1)
+    case.k[:300, 0, :16] *= 1e-12                                          # request 0, the first key head
+    _, planes = on_device(case)
+    table = case.table.clone()
+    gone = 40 // page                                                      # request 1: one page of it, of every head
+    table[1, gone] = -1
+    k, v = case.held()
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(sum(new), heads, dim, generator=g)
+    q[:150, :heads // kv_heads, :16] *= 1e12
+    q = q.flatten(1).to(BF16)
+    sink = torch.randn(heads, generator=g) if with_sink else None
+    scale, starts = dim ** -0.5, [0, 150, 350, 351]
+    wide = torch.zeros(351, heads * dim + 3, dtype=BF16, device=DEV)
+    wide[:, 3:] = q.to(DEV)
+    sinks = None if sink is None else sink.to(DEV)
+    rows = torch.full((351, heads * dim + 5), 9.0, dtype=out_dtype, device=DEV)
+    ops.packed_attention_prompts(wide[:, 3:], rows[:, :heads * dim], *planes, ints(starts), ints(lengths), table.to(DEV), ints([0, 1, 2]), 0, 3, 3 + 4 + 1, 300, heads, kv_heads,
+                                 dim, page, window, scale, softcap=softcap, sink=sinks, shares=shares)
+    single = torch.full((351, heads * dim + 5), 9.0, dtype=out_dtype, device=DEV)
+    positions = [*range(150, 300), *range(200), 0]
+    ops.packed_attention_tokens(wide[:, 3:], single[:, :heads * dim], *planes, ints([0] * 150 + [1] * 200 + [2]), ints(positions), table.to(DEV), heads, kv_heads, dim, page,
+                                window, scale, 300, softcap=softcap, sink=sinks, shares=shares)
+    for out in (rows, single):
+        assert (out[:, heads * dim:] == 9.0).all()
+        got = out[:, :heads * dim].cpu().double().view(351, heads, dim)
+        for item in (0, 2):
+            part = slice(starts[item], starts[item + 1])
+            found = attention(q[part].double().view(-1, heads, dim), case.context(item, k), case.context(item, v), torch.arange(lengths[item] - new[item], lengths[item]), scale,
+                              window, softcap, sink)
+            agrees(got[part], found, limit_of(found, scale, BF16, dim))
+        keys, values = case.context(1, k), case.context(1, v)
+        for at in (0, 39, 63, 64, 128, 199):
+            seen = torch.tensor([i for i in range(at + 1) if i // page != gone
+                                 and (not window or (at - i < window if window > 0 else i // -window == at // -window))], dtype=torch.long)
+            if not len(seen):
+                assert (got[150 + at] == 0).all()
+                continue
+            found = attention(q[150 + at:151 + at].double().view(1, heads, dim), keys[seen], values[seen], torch.tensor([len(seen) - 1]), scale, None, softcap, sink)
+            agrees(got[150 + at:151 + at], found, limit_of(found, scale, BF16, dim))
+
+
+@pytest.mark.parametrize("dim", [20, 64, 128])
+@pytest.mark.parametrize("k_scale,v_scale,q_scale", [(1.0, 3e30, 1.0), (3e5, 1.0, 2e5), (1.0, 1e-3, 1e20)])
+def test_large_numbers_in_prompts_in_float32(dim, k_scale, v_scale, q_scale):
+    ops, heads, length, new = ops_for(F32), 2, 200, 150
+    case = PackedCase([length], heads, dim, 16, F32, seed=4)
+    case.k, case.v = case.k * k_scale, case.v * v_scale
+    _, planes = on_device(case)
+    k, v = (x.double() for x in case.held())
+    q = torch.randn(new, heads * dim, generator=torch.Generator().manual_seed(2)) * q_scale
+    scale = 0.125 / max(1.0, k_scale * q_scale)
+    found = attention(q.double().view(new, heads, dim), k, v, torch.arange(length - new, length), scale)
+    agrees(prompts(ops, case, planes, q, new, heads, scale), found, limit_of(found, scale, F32, dim))
